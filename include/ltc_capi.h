@@ -289,6 +289,131 @@ int ltc_ode_unfold_bwd(const float* v_buffer, const float* w_pos, const float* w
                        void* workspace, long long workspace_bytes, void* stream);
 
 /*
+ * Sequence and token operators. No counterpart in the reference: a recurrence
+ * whose time axis is parallel, and what turns a layer's outputs into token
+ * scores and training losses. Tensors are fp32, bf16 or fp16 (LTC_F32, LTC_BF16,
+ * LTC_F16), unit stride along their last dimension, any alignment their type
+ * has; states, sums and statistics are fp32. Results are deterministic.
+ */
+#define LTC_F32 0
+#define LTC_BF16 1
+#define LTC_F16 2
+
+/* Gate forms: a = sigmoid(gate), h = a h + (1 - a) x; a = exp(gate), h = a h + x.
+ * exp(gate) over 1 is taken as it is: the product of the decays of up to 256
+ * tokens has to stay in fp32's range then. */
+#define LTC_GATE_BLEND 0
+#define LTC_GATE_DECAY 1
+
+/*
+ * Gated linear recurrence over B sequences of T steps, or, with cu_seqlens
+ * (B + 1 ascending int32 boundaries on the device), over B packed sequences of T
+ * tokens in all: sequence s is tokens cu_seqlens[s] up to cu_seqlens[s + 1], and
+ * may be empty. Tokens outside every sequence give zeros, in out and in the
+ * gradients. Boundaries outside 0 ... T or out of order give unspecified results
+ * without an access out of range.
+ *   x            (B,T,H) with element strides sxb, sxt; packed (T,H), stride sxt
+ *   gate         likewise; its type is x's or LTC_F32
+ *   state        (B,H) fp32 contiguous, or NULL for zero
+ *   out          (B,T,H) or (T,H), x's type, contiguous
+ *   state_final  (B,H) fp32: the last state; an empty sequence's initial one
+ *   saved        ltc_gated_scan_saved_floats() floats, written when save is
+ *                nonzero, for the backward of the same x, gate, state, cu_seqlens
+ */
+long long ltc_gated_scan_saved_floats(int B, int T, int H, int packed);
+long long ltc_gated_scan_fwd_workspace_bytes(int B, int T, int H, int packed);
+long long ltc_gated_scan_bwd_workspace_bytes(int B, int T, int H, int packed);
+int ltc_gated_scan_forward(const void* x, long long sxb, long long sxt, const void* gate,
+                           long long sgb, long long sgt, const float* state,
+                           const int* cu_seqlens, int x_type, int gate_type, int form, int B,
+                           int T, int H, int save, void* out, float* state_final, float* saved,
+                           void* workspace, long long workspace_bytes, void* stream);
+
+/*
+ * Its backward. grad_out (NULL for zero) has x's shape and type and strides sob,
+ * sot; grad_state_final (B,H) fp32 contiguous or NULL for zero. grad_x (x's type),
+ * grad_gate (the gate's) and grad_state (B,H) fp32 are contiguous; each may be
+ * NULL where it is not wanted.
+ */
+int ltc_gated_scan_backward(const void* x, long long sxb, long long sxt, const void* gate,
+                            long long sgb, long long sgt, const float* state,
+                            const int* cu_seqlens, int x_type, int gate_type, int form, int B,
+                            int T, int H, const float* saved, const void* grad_out,
+                            long long sob, long long sot, const float* grad_state_final,
+                            void* grad_x, void* grad_gate, float* grad_state, void* workspace,
+                            long long workspace_bytes, void* stream);
+
+/*
+ * One token of B streams: out[b] and the stream's new state, written over the old.
+ *   x, gate      (B,H), row strides sxb, sgb
+ *   state        (P,H) fp32, row stride ssp (at least H)
+ *   slots        int32 (B): the row of state of each row, or NULL for row b (P = B).
+ *                A negative slot is padding: its row of out is zero and no state is
+ *                touched. A slot of P or more gives a row of NaN. Rows that name the
+ *                same slot are taken in their order, as tokens of one stream.
+ *   out          (B,H), x's type, contiguous
+ */
+int ltc_gated_scan_step(const void* x, long long sxb, const void* gate, long long sgb,
+                        float* state, long long ssp, const int* slots, int x_type,
+                        int gate_type, int form, int B, int H, int P, void* out, void* stream);
+
+/*
+ * Log probabilities of given tokens under softmax(logits / temperature), the
+ * distribution's entropy, and its `top` most probable tokens.
+ *   logits       (N,V), row stride sl
+ *   ids          (N) int32 or (ids64 nonzero) int64. A negative id is a row without
+ *                a token: log probability and entropy 0, gradient 0. An id of V or
+ *                more gives NaN.
+ *   logp, entropy   (N) fp32; entropy may be NULL
+ *   top_logp, top_ids   (N,top) fp32 and int64, most probable first, equal logits by
+ *                the lower id; every row, with a token or not. top <= LTC_TOP_MAX
+ *                and <= V; 0 for none
+ *   stats        (N,3) fp32 for the backward, or NULL
+ * A logit of -inf has probability 0; a row of nothing else, or with a NaN or +inf,
+ * gives NaN (in such a row top_ids are in range, but otherwise unspecified).
+ */
+#define LTC_TOP_MAX 32
+long long ltc_token_logprobs_workspace_bytes(long long N, int V, int top, int logits_type);
+int ltc_token_logprobs_forward(const void* logits, long long sl, const void* ids, int ids64,
+                               int logits_type, long long N, int V, int top, float temperature,
+                               float* logp, float* entropy, float* top_logp, long long* top_ids,
+                               float* stats, void* workspace, long long workspace_bytes,
+                               void* stream);
+/* grad_logp, grad_entropy: (N) fp32 with strides slp, sen, or NULL for zero;
+ * grad_logits (N,V) contiguous, the logits' type. */
+int ltc_token_logprobs_backward(const void* logits, long long sl, const void* ids, int ids64,
+                                int logits_type, long long N, int V, float temperature,
+                                const float* stats, const float* grad_logp, long long slp,
+                                const float* grad_entropy, long long sen, void* grad_logits,
+                                void* stream);
+
+/*
+ * Distillation from a teacher's top logits:
+ *   loss = temperature^2 sum_k p_k (log p_k - log q[teacher_ids[k]]),
+ * p the softmax of the row's teacher_logits / temperature over the entries that are
+ * there, q = softmax(logits / temperature) over the vocabulary.
+ *   teacher_logits  (N,K), row stride st; any of the types
+ *   teacher_ids     (N,K) int32 or int64, row stride si; a negative id is an entry
+ *                that is not there, one of V or more gives NaN. An id may come twice.
+ *                1 <= K <= LTC_TEACHER_MAX
+ *   loss         (N) fp32; 0 for a row without entries, or whose entries' logits are
+ *                all -inf
+ * The backward gives dL/dlogits from grad_loss (N), stride sgl; the teacher gets none.
+ */
+#define LTC_TEACHER_MAX 1024
+long long ltc_top_distill_workspace_bytes(long long N, int V, int logits_type);
+int ltc_top_distill_forward(const void* logits, long long sl, const void* teacher_logits,
+                            long long st, const void* teacher_ids, long long si, int ids64,
+                            int logits_type, int teacher_type, long long N, int V, int K,
+                            float temperature, float* loss, float* stats, void* workspace,
+                            long long workspace_bytes, void* stream);
+int ltc_top_distill_backward(const void* logits, long long sl, const void* teacher_logits,
+                             long long st, const void* teacher_ids, long long si, int ids64,
+                             int logits_type, int teacher_type, long long N, int V, int K,
+                             float temperature, const float* stats, const float* grad_loss,
+                             long long sgl, void* grad_logits, void* stream);
+
+/*
  * Launch plan of one call, for diagnostics and host-side bounds tests. No
  * counterpart in the reference. Writes up to n of: Hp, Dp, NB (batch rows
  * per ODE workgroup), KS (reduction split), RC (= Hp/KS), threads per ODE

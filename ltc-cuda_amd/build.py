@@ -18,7 +18,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_NAME = "libltc_hip.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
-SOURCES = ("ltc_device.hip", "ltc_capi.hip")
+SOURCES = ("ltc_device.hip", "ltc_capi.hip", "ltc_scan_device.hip", "ltc_token_device.hip",
+           "ltc_seq_capi.hip")
 ARCH = os.environ.get("LTC_OFFLOAD_ARCH", "gfx950")
 
 
@@ -33,7 +34,8 @@ def source_files() -> list:
     """Every file the library and the torch extension are built from."""
     inc = os.path.join(os.path.dirname(HERE), "include", "ltc_capi.h")
     return [os.path.join(CSRC, s) for s in SOURCES] + [
-        os.path.join(CSRC, "ltc_internal.h"), os.path.join(CSRC, "ltc_torch_ext.cpp"), inc]
+        os.path.join(CSRC, "ltc_internal.h"), os.path.join(CSRC, "ltc_seq_internal.h"),
+        *[os.path.join(CSRC, s) for s in EXT_SOURCES], inc]
 
 
 def command(out: str = LIB_PATH, arch: str = ARCH) -> list:
@@ -58,7 +60,7 @@ def command(out: str = LIB_PATH, arch: str = ARCH) -> list:
     ]
 
 
-EXT_SRC = os.path.join(CSRC, "ltc_torch_ext.cpp")
+EXT_SOURCES = ("ltc_torch_ext.cpp", "ltc_torch_seq.cpp")
 EXT_NAME = "_ltc_torch"
 
 
@@ -68,8 +70,8 @@ def ext_path() -> str:
 
 
 def ext_command(out: str) -> list:
-    """Host-only C++ build of the torch glue (the autograd node of the
-    fused module path), linked against libltc_hip.so through $ORIGIN."""
+    """Host-only C++ build of the torch glue (the autograd nodes of the fused
+    module path and of the sequence and token operators), linked against libltc_hip.so through $ORIGIN."""
     import sysconfig
     import torch
     from torch.utils import cpp_extension as ce
@@ -83,7 +85,7 @@ def ext_command(out: str) -> list:
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}", f"-DTORCH_EXTENSION_NAME={EXT_NAME}",
         "-DTORCH_API_INCLUDE_EXTENSION_H",
-        *[f"-I{d}" for d in incs], EXT_SRC, "-o", out,
+        *[f"-I{d}" for d in incs], *[os.path.join(CSRC, s) for s in EXT_SOURCES], "-o", out,
         f"-L{HERE}", "-lltc_hip", *[f"-L{d}" for d in libs],
         "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python",
         "-Wl,-rpath,$ORIGIN", "-Wl,--no-as-needed",

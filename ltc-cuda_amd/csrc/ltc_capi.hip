@@ -12,6 +12,7 @@
 
 #include "../../include/ltc_capi.h"
 #include "ltc_internal.h"
+#include "ltc_seq_internal.h"
 
 // Scratch of the no-allocation forward (ltc_full_forward_noalloc): one array
 // per device, held until the process ends. In host code `scratch` names a
@@ -709,7 +710,10 @@ int check_dims(int B, int T, int D, int H, int U) {
 // ---------------------------------------------------------------------------
 const char* const kNames[ltc::K_COUNT] = {"ltc_prep",     "ltc_sens_fwd", "ltc_ode_fwd",
                                           "ltc_ode_bwd",  "ltc_rec_grad", "ltc_sens_bwd",
-                                          "ltc_ln_bwd",   "ltc_finalize"};
+                                          "ltc_ln_bwd",   "ltc_finalize",
+                                          "ltc_scan_fwd", "ltc_scan_bwd", "ltc_scan_step",
+                                          "ltc_logprobs_fwd", "ltc_logprobs_bwd",
+                                          "ltc_distill_fwd", "ltc_distill_bwd"};
 
 struct Timing {
   std::mutex mu;
@@ -909,6 +913,16 @@ void* noalloc_scratch() {
 }
 
 }  // namespace
+
+// The same services for the entry points of ltc_seq_capi.hip.
+namespace ltc {
+int host_fail(int code, const std::string& msg) { return fail(code, msg); }
+int host_hip_fail(const char* what, hipError_t e) { return hip_fail(what, e); }
+void host_clear_error() { g_err.clear(); }
+hipError_t host_timed(int id, hipError_t (*launch)(void*), void* ctx) {
+  return timed(id, nullptr, [&] { return launch(ctx); });
+}
+}  // namespace ltc
 
 extern "C" {
 

@@ -59,6 +59,13 @@ enum KernelId : int {
   K_SENS_BWD,
   K_LN_BWD,
   K_FINALIZE,
+  K_SCAN_FWD,
+  K_SCAN_BWD,
+  K_SCAN_STEP,
+  K_LOGPROBS_FWD,
+  K_LOGPROBS_BWD,
+  K_DISTILL_FWD,
+  K_DISTILL_BWD,
   K_COUNT
 };
 

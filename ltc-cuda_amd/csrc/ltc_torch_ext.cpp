@@ -220,8 +220,12 @@ std::vector<Tensor> module_apply(const Tensor& x, const c10::optional<Tensor>& s
 
 }  // namespace
 
+// csrc/ltc_torch_seq.cpp
+void bind_sequence_operators(pybind11::module_& m);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "LTC fused module path: autograd node over libltc_hip.so";
   m.def("module_apply", &module_apply, "Fused LTC layer forward (autograd-aware)");
+  bind_sequence_operators(m);
   m.def("abi_version", &ltc_abi_version, "ABI version of the loaded libltc_hip.so");
 }

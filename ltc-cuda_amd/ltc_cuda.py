@@ -70,6 +70,12 @@ class CApi:
         "ltc_sensory_bwd_workspace_bytes", "ltc_sensory_bwd",
         "ltc_ode_unfold_bwd_workspace_bytes", "ltc_ode_unfold_bwd",
         "ltc_full_forward_noalloc", "ltc_device_status", "ltc_set_cluster_spin_ticks",
+        "ltc_gated_scan_saved_floats", "ltc_gated_scan_fwd_workspace_bytes",
+        "ltc_gated_scan_bwd_workspace_bytes", "ltc_gated_scan_forward",
+        "ltc_gated_scan_backward", "ltc_gated_scan_step",
+        "ltc_token_logprobs_workspace_bytes", "ltc_token_logprobs_forward",
+        "ltc_token_logprobs_backward", "ltc_top_distill_workspace_bytes",
+        "ltc_top_distill_forward", "ltc_top_distill_backward",
     )
     PLAN_FIELDS = ("Hp", "Dp", "NB", "KS", "RC", "threads", "lds_fwd", "lds_bwd", "NCH",
                    "NRC", "ode_workgroups", "fuse", "KSB", "RCB",
@@ -150,6 +156,42 @@ class CApi:
         lib.ltc_ode_unfold_bwd.argtypes = (
             [_f32p] * 11 + [_int, _int, _int, _flt] + [_f32p] * 10
             + [_f32p, _i64, ctypes.c_void_p])
+        for name in ("ltc_gated_scan_saved_floats", "ltc_gated_scan_fwd_workspace_bytes",
+                     "ltc_gated_scan_bwd_workspace_bytes"):
+            fn = getattr(lib, name)
+            fn.restype = _i64
+            fn.argtypes = [_int, _int, _int, _int]
+        _scan = [_f32p, _i64, _i64, _f32p, _i64, _i64, _f32p, _f32p] + [_int] * 6
+        lib.ltc_gated_scan_forward.restype = _int
+        lib.ltc_gated_scan_forward.argtypes = (
+            _scan + [_int, _f32p, _f32p, _f32p, _f32p, _i64, ctypes.c_void_p])
+        lib.ltc_gated_scan_backward.restype = _int
+        lib.ltc_gated_scan_backward.argtypes = (
+            _scan + [_f32p, _f32p, _i64, _i64, _f32p, _f32p, _f32p, _f32p, _f32p, _i64,
+                     ctypes.c_void_p])
+        lib.ltc_gated_scan_step.restype = _int
+        lib.ltc_gated_scan_step.argtypes = (
+            [_f32p, _i64, _f32p, _i64, _f32p, _i64, _f32p] + [_int] * 6
+            + [_f32p, ctypes.c_void_p])
+        lib.ltc_token_logprobs_workspace_bytes.restype = _i64
+        lib.ltc_token_logprobs_workspace_bytes.argtypes = [_i64, _int, _int, _int]
+        lib.ltc_token_logprobs_forward.restype = _int
+        lib.ltc_token_logprobs_forward.argtypes = (
+            [_f32p, _i64, _f32p, _int, _int, _i64, _int, _int, _flt] + [_f32p] * 6
+            + [_i64, ctypes.c_void_p])
+        lib.ltc_token_logprobs_backward.restype = _int
+        lib.ltc_token_logprobs_backward.argtypes = (
+            [_f32p, _i64, _f32p, _int, _int, _i64, _int, _flt, _f32p, _f32p, _i64, _f32p, _i64,
+             _f32p, ctypes.c_void_p])
+        lib.ltc_top_distill_workspace_bytes.restype = _i64
+        lib.ltc_top_distill_workspace_bytes.argtypes = [_i64, _int, _int]
+        _dist = [_f32p, _i64, _f32p, _i64, _f32p, _i64, _int, _int, _int, _i64, _int, _int, _flt]
+        lib.ltc_top_distill_forward.restype = _int
+        lib.ltc_top_distill_forward.argtypes = (
+            _dist + [_f32p, _f32p, _f32p, _i64, ctypes.c_void_p])
+        lib.ltc_top_distill_backward.restype = _int
+        lib.ltc_top_distill_backward.argtypes = (
+            _dist + [_f32p, _f32p, _i64, _f32p, ctypes.c_void_p])
         lib.ltc_device_status.restype = _int
         lib.ltc_device_status.argtypes = [_int]
         lib.ltc_set_cluster_spin_ticks.restype = _i64
@@ -807,6 +849,87 @@ def ltc_cuda_forward(x_seq, state, w_pos, w_erev, mu, sigma,
         x_seq, state, w_pos, w_erev, mu, sigma,
         sensory_mu, sensory_sigma, sensory_erev, sensory_w_pos,
         cm_t, gleak_pos, vleak, ode_unfolds, epsilon, needs_grad)
+
+
+# ------------------------------------------------ sequence and token operators
+
+# ltc_gated_scan's gates, as include/ltc_capi.h numbers them.
+GATE_FORMS = {"blend": 0, "decay": 1}
+
+
+def _require_ext():
+    require_kernels()
+    if _torch_ext is None:
+        raise RuntimeError("the LTC torch extension is not built: run `python "
+                           f"{os.path.join(PKG_DIR, 'build.py')}`")
+    return _torch_ext
+
+
+def _gate_form(form: str) -> int:
+    if form not in GATE_FORMS:
+        raise ValueError(f"form must be one of {sorted(GATE_FORMS)}, got {form!r}")
+    return GATE_FORMS[form]
+
+
+def ltc_gated_scan(x, gate, state=None, cu_seqlens=None, form="blend"):
+    """Gated linear recurrence over whole sequences -> (out, state_final).
+
+    form "blend": a = sigmoid(gate), h_t = a_t h_{t-1} + (1 - a_t) x_t, the update
+    of an LTC neuron without recurrent synapses (a = cm / (cm + conductances), x
+    the potential they drive it to). form "decay": a = exp(gate), h_t = a_t h_{t-1}
+    + x_t; gates over 0 are taken as they are, and overflow where their product
+    over 256 tokens does.
+
+    x       (B, T, H), float32, bfloat16 or float16; with cu_seqlens (tokens, H)
+    gate    x's shape; its type is x's or float32
+    state   (B, H) float32, or None for zero
+    cu_seqlens  int32 (sequences + 1,) on the device, ascending: sequence s is
+            tokens cu_seqlens[s] up to cu_seqlens[s + 1]. Sequences may be empty
+            (their state comes back); tokens outside all of them give zeros, in
+            out and in the gradients.
+    out     x's shape and type; state_final (B, H) float32.
+
+    States are float32 throughout. Gradients reach x, gate and state through both
+    outputs. Time is parallel: a long sequence costs its bytes, not its steps.
+    """
+    return tuple(_require_ext().gated_scan(x, gate, state, cu_seqlens, _gate_form(form)))
+
+
+def ltc_gated_scan_step(x, gate, state, slots=None, form="blend"):
+    """One token of each stream: returns out (B, H) and updates `state` in place.
+
+    x, gate  (B, H) as in ltc_gated_scan; state (B, H) float32, or with slots
+    (int32 (B,)) a pool (P, H) whose row slots[b] is row b's. A negative slot is a
+    padding row: zeros come out and no state is touched; a slot of P or more gives
+    NaN. Rows that name one slot are taken in their order, as tokens of one
+    stream. No backward: it raises where a gradient would be wanted.
+    """
+    return _require_ext().gated_scan_step(x, gate, state, slots, _gate_form(form))
+
+
+def ltc_token_logprobs(logits, ids, top=0, temperature=1.0):
+    """Log probabilities of given tokens under softmax(logits / temperature).
+
+    logits (..., V), ids (...) int32 or int64 -> (logp (...), entropy (...)), with
+    top > 0 also (top_logp (..., top), top_ids (..., top) int64): the most probable
+    tokens, equal logits by the lower id. All but the ids are float32. Rows with a
+    negative id have no token: 0 and 0, and no gradient; an id of V or more gives
+    NaN. Logits of -inf have probability 0. Gradients reach logits through logp and
+    entropy; the alternatives carry none.
+    """
+    return tuple(_require_ext().token_logprobs(logits, ids, int(top), float(temperature)))
+
+
+def ltc_top_distill(logits, teacher_logits, teacher_ids, temperature=1.0):
+    """Distillation loss of each row against a teacher's K best logits -> (...) float32.
+
+    temperature^2 sum_k p_k (log p_k - log q[teacher_ids_k]), with p the softmax of
+    teacher_logits (..., K) / temperature over the entries that are there (a
+    negative id is one that is not) and q = softmax(logits (..., V) / temperature).
+    K <= 1024. A row without entries gives 0 and no gradient; an id of V or more
+    gives NaN. Gradients reach logits only; the teacher's have to be detached.
+    """
+    return _require_ext().top_distill(logits, teacher_logits, teacher_ids, float(temperature))
 
 
 def _detach_tree(obj):
