@@ -5,13 +5,16 @@
 //   decay: dL/dx = d,         dL/dg = d h_{t-1} a
 //
 // A run of tokens maps the state that enters it affinely, h -> A h + B, and two
-// runs compose to (A2 A1, A2 B1 + B2), so time is cut into tiles: each tile's
-// map, then what enters every tile, then every tile's tokens. The tokens of all
+// runs compose to (A2 A1, A2 B1 + B2), so time is cut into tiles: a workgroup
+// reads its tile once, leaves its map for the tiles behind it, takes what enters
+// it from the maps before, and runs its tokens out of its registers. The tokens of all
 // sequences lie end to end; a sequence's first token gives a h0 + u whatever comes
 // from before. Decays are never negative, so a map whose A has the sign bit set
 // stands for one that drops what enters it, NaN and infinities too. All maps and states are fp32; out and the
 // gradients are rounded to their type once, when they are stored.
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "../../include/ltc_capi.h"
 #include "ltc_seq_internal.h"
@@ -25,9 +28,38 @@ constexpr float kLog2e = 1.4426950408889634f;
 // else 4 * sequence + 1 for its first token + 2 for its last.
 constexpr int kMarkNone = -1, kMarkStart = 1, kMarkEnd = 2;
 
+// V values of a type, kept packed in words of 32 bits.
 template <class T, int V>
 struct Vec {
-  T v[V];
+  static constexpr int kWords = V * (int)sizeof(T) / 4;
+  static_assert(kWords * 4 == V * (int)sizeof(T), "whole words");
+  unsigned w[kWords];
+
+  __device__ __forceinline__ float get(int v) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[v]);
+    } else if constexpr (std::is_same<T, __bf16>::value) {
+      return __uint_as_float(v & 1 ? w[v / 2] & 0xffff0000u : w[v / 2] << 16);
+    } else {
+      const unsigned short h = (unsigned short)(v & 1 ? w[v / 2] >> 16 : w[v / 2]);
+      return (float)__builtin_bit_cast(_Float16, h);
+    }
+  }
+  // Rounded to nearest, ties to even; the packed conversions take two.
+  __device__ __forceinline__ void put(const float (&f)[V]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) w[v] = __float_as_uint(f[v]);
+    } else {
+      typedef float F2 __attribute__((ext_vector_type(2)));
+      typedef T T2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+      for (int v = 0; v < V; v += 2) {
+        const F2 q = {f[v], f[v + 1]};
+        w[v / 2] = __builtin_bit_cast(unsigned, __builtin_convertvector(q, T2));
+      }
+    }
+  }
 };
 
 // n (< V: the row's last channels) of V values at p, which has T's alignment
@@ -36,10 +68,16 @@ template <class T, int V>
 __device__ __forceinline__ Vec<T, V> load_vec(const T* p, int n) {
   Vec<T, V> r;
   if (n >= V) {
-    __builtin_memcpy(&r, p, sizeof(r));
+    __builtin_memcpy(r.w, p, sizeof(r.w));
   } else {
 #pragma unroll
-    for (int v = 0; v < V; ++v) r.v[v] = v < n ? p[v] : T(0.f);
+    for (int i = 0; i < Vec<T, V>::kWords; ++i) r.w[i] = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (v < n) {
+        if constexpr (sizeof(T) == 4) r.w[v] = reinterpret_cast<const unsigned*>(p)[v];
+        else r.w[v / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(p)[v] << (v & 1) * 16;
+      }
   }
   return r;
 }
@@ -47,70 +85,73 @@ __device__ __forceinline__ Vec<T, V> load_vec(const T* p, int n) {
 template <class T, int V>
 __device__ __forceinline__ void store_vec(T* p, const Vec<T, V>& r, int n) {
   if (n >= V) {
-    __builtin_memcpy(p, &r, sizeof(r));
+    __builtin_memcpy(p, r.w, sizeof(r.w));
   } else {
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      if (v < n) p[v] = r.v[v];
+      if (v < n) {
+        if constexpr (sizeof(T) == 4) reinterpret_cast<unsigned*>(p)[v] = r.w[v];
+        else reinterpret_cast<unsigned short*>(p)[v] = (unsigned short)(r.w[v / 2] >> (v & 1) * 16);
+      }
   }
 }
 
-// a and 1 - a (decay: 1), each to its own relative precision: sigmoid from
-// exp(-|g|), which does not overflow. A NaN a has no sign either.
+// a and 1 - a (decay: 1), each to its own relative precision: with e = exp(-g),
+// a = 1 / (1 + e) and 1 - a = e a. e is kept below 2^126, where a is 2^-126 and
+// 1 - a is 1; `minimum` passes a NaN on.
 template <int FORM>
 __device__ __forceinline__ void gate_of(float g, float& a, float& na) {
   if constexpr (FORM == LTC_GATE_BLEND) {
-    const float e = __builtin_amdgcn_exp2f(-fabsf(g) * kLog2e);
-    const float r = __builtin_amdgcn_rcpf(1.f + e);
-    const float lo = e * r;
-    a = fabsf(g < 0.f ? lo : r);
-    na = g < 0.f ? r : lo;
+    const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(g * -kLog2e, 126.f));
+    a = __builtin_amdgcn_rcpf(1.f + e);
+    na = e * a;
   } else {
-    a = fabsf(__builtin_amdgcn_exp2f(g * kLog2e));
+    a = __builtin_amdgcn_exp2f(g * kLog2e);
     na = 1.f;
   }
 }
 
-// Where a thread's tokens lie and what they are: bit i of the masks is token i.
+// A thread's tokens: bit i of the masks is token i. Tokens outside all sequences
+// (valid 0) drop what comes before them, as a sequence's first does.
 template <int LT>
 struct Tokens {
-  long long t0;           // first token
+  int t0;         // first token
   unsigned valid, start, end;
-  int b[LT];              // sequence of token i
-  int r[LT];              // uniform batches: step of token i in its sequence
+  unsigned wrap;  // uniform batches: the next token is another sequence's
+  int b[LT];      // sequence of token i
+  long long off_b, off_t;  // uniform batches: sequence and step of the first token
 };
 
 template <int LT, bool PACKED>
-__device__ __forceinline__ Tokens<LT> tokens_of(const ScanArgs& p, long long t0) {
+__device__ __forceinline__ Tokens<LT> tokens_of(const ScanArgs& p, int t0) {
   Tokens<LT> k;
   k.t0 = t0;
-  k.valid = k.start = k.end = 0;
+  k.valid = k.start = k.end = k.wrap = 0;
   int b = 0, r = 0;
   if constexpr (!PACKED) {
-    b = (int)(t0 / p.T);
-    r = (int)(t0 - (long long)b * p.T);
+    b = (int)((unsigned)t0 / (unsigned)p.T);
+    r = t0 - b * p.T;
   }
+  k.off_b = b;
+  k.off_t = r;
 #pragma unroll
   for (int i = 0; i < LT; ++i) {
     const bool in = t0 + i < p.N;
     if constexpr (PACKED) {
       const int m = in ? p.marks[t0 + i] : kMarkNone;
       k.b[i] = m >> 2;
-      k.r[i] = 0;
       if (m >= 0) {
         k.valid |= 1u << i;
-        if (m & kMarkStart) k.start |= 1u << i;
         if (m & kMarkEnd) k.end |= 1u << i;
       }
+      if (m < 0 || (m & kMarkStart)) k.start |= 1u << i;
     } else {
       k.b[i] = b;
-      k.r[i] = r;
-      if (in) {
-        k.valid |= 1u << i;
-        if (r == 0) k.start |= 1u << i;
-        if (r == p.T - 1) k.end |= 1u << i;
-      }
+      if (in) k.valid |= 1u << i;
+      if (!in || r == 0) k.start |= 1u << i;
       if (++r == p.T) {
+        if (in) k.end |= 1u << i;
+        k.wrap |= 1u << i;
         r = 0;
         ++b;
       }
@@ -119,90 +160,70 @@ __device__ __forceinline__ Tokens<LT> tokens_of(const ScanArgs& p, long long t0)
   return k;
 }
 
-// Element offset of token i's row.
-template <bool PACKED, int LT>
-__device__ __forceinline__ long long row_of(const Tokens<LT>& k, int i, long long sb, long long st) {
-  if constexpr (PACKED) return (k.t0 + i) * st;
-  else return k.b[i] * sb + k.r[i] * st;
+// First and last token of packed token t's sequence s, whatever the boundaries.
+__device__ __forceinline__ int begin_of(const ScanArgs& p, int s, int t) {
+  const int q = p.cu[s];
+  return q < 0 || q > t ? t : q;
+}
+__device__ __forceinline__ int end_of(const ScanArgs& p, int s, int t) {
+  const long long q = (long long)p.cu[s + 1] - 1;
+  return q >= p.N ? (int)p.N - 1 : q < t ? t : (int)q;
 }
 
-// A thread's tokens, loaded.
-template <class T, class G, int V, int LT>
-struct Loaded {
-  Vec<T, V> x[LT];
-  Vec<G, V> g[LT];
-};
-
-template <class T, class G, int V, int LT, bool PACKED>
-__device__ __forceinline__ void load_tokens(const ScanArgs& p, const Tokens<LT>& k, int ch, int n,
-                                            Loaded<T, G, V, LT>& d) {
+// n channels of the thread's tokens from a tensor of element strides sb, st; zero
+// where there are none.
+template <class T, int V, int LT, bool PACKED>
+__device__ __forceinline__ void load_tokens(const void* base, long long sb, long long st, const ScanArgs& p,
+                                            const Tokens<LT>& k, int ch, int n, Vec<T, V> (&d)[LT]) {
+  const T* q = static_cast<const T*>(base) + ch;
+  long long jump = 0;
+  if constexpr (PACKED) {
+    q += k.t0 * st;
+  } else {
+    q += k.off_b * sb + k.off_t * st;
+    jump = sb - p.T * st;
+  }
 #pragma unroll
   for (int i = 0; i < LT; ++i) {
-    if (n > 0 && (k.valid >> i & 1)) {
-      d.x[i] = load_vec<T, V>(static_cast<const T*>(p.x) + row_of<PACKED>(k, i, p.sxb, p.sxt) + ch, n);
-      d.g[i] = load_vec<G, V>(static_cast<const G*>(p.g) + row_of<PACKED>(k, i, p.sgb, p.sgt) + ch, n);
-    } else {
-      d.x[i] = Vec<T, V>{};
-      d.g[i] = Vec<G, V>{};
-    }
+    d[i] = Vec<T, V>{};
+    if (base != nullptr && n > 0 && (k.valid >> i & 1)) d[i] = load_vec<T, V>(q, n);
+    q += st;
+    if (!PACKED && (k.wrap >> i & 1)) q += jump;
   }
 }
 
-// Initial state of token i's sequence.
+// h = the state that enters token i of the thread, where it drops what comes
+// before: its sequence's initial one, or 0.
 template <int V, int LT>
-__device__ __forceinline__ Vec<float, V> state_of(const ScanArgs& p, const Tokens<LT>& k, int i, int ch,
-                                                  int n) {
-  if (p.h0 == nullptr || n <= 0) return Vec<float, V>{};
-  return load_vec<float, V>(p.h0 + (long long)k.b[i] * p.H + ch, n);
+__device__ __forceinline__ void begin_state(const ScanArgs& p, const Tokens<LT>& k, int i, int ch, int n,
+                                            float (&h)[V]) {
+  Vec<float, V> q{};
+  if (p.h0 != nullptr && n > 0 && (k.valid >> i & 1))
+    q = load_vec<float, V>(p.h0 + (long long)k.b[i] * p.H + ch, n);
+#pragma unroll
+  for (int v = 0; v < V; ++v) h[v] = q.get(v);
 }
 
 // Whether a map drops what enters it, and what leaves one, h having entered.
 __device__ __forceinline__ bool drops(float A) { return __float_as_int(A) < 0; }
 __device__ __forceinline__ float leave(float A, float B, float h) { return drops(A) ? B : fmaf(A, h, B); }
 
-// Token i's map (a, u) of every channel; a sequence's first token takes its
-// initial state in and drops what comes from before (a = -1), as does a token
-// outside all sequences, which gives 0.
-template <int FORM, class T, class G, int V, int LT>
-__device__ __forceinline__ void maps_of(const ScanArgs& p, const Tokens<LT>& k,
-                                        const Loaded<T, G, V, LT>& d, int i, int ch, int n,
-                                        float (&a)[V], float (&u)[V]) {
-  const bool valid = k.valid >> i & 1;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    float na;
-    gate_of<FORM>((float)d.g[i].v[v], a[v], na);
-    u[v] = na * (float)d.x[i].v[v];
-    if (!valid) {
-      a[v] = -1.f;
-      u[v] = 0.f;
-    }
-  }
-  if (k.start >> i & 1) {
-    const Vec<float, V> h0 = state_of<V>(p, k, i, ch, n);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      u[v] = fmaf(a[v], h0.v[v], u[v]);
-      a[v] = -1.f;
-    }
-  }
-}
-
 // A workgroup's exchange of its slots' maps: each slot leaves the map of its
 // tokens, and every slot gets the map of all slots before it.
-template <int CB>
+template <int CB, int THREADS>
 struct SlotMaps {
-  static constexpr int kParts = kScanThreads / CB;  // threads per channel
+  static constexpr int kParts = THREADS / CB;  // threads per channel
   static constexpr int kPer = kScanSlots / kParts;  // slots per thread
-  static_assert(kParts * CB == kScanThreads && kPer * kParts == kScanSlots, "slot split");
+  static_assert(kParts * CB == THREADS && kPer * kParts == kScanSlots, "slot split");
   float a[kScanSlots][CB], b[kScanSlots][CB];
   float pa[kParts][CB], pb[kParts][CB];
 
   template <int V>
-  __device__ __forceinline__ void put(int slot, int c, const float (&A)[V], const float (&B)[V]) {
+  __device__ __forceinline__ void put(int slot, int c, const float (&A)[V], const float (&B)[V],
+                                      bool dropped) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      a[slot][c * V + v] = A[v];
+      a[slot][c * V + v] = dropped ? -1.f : fabsf(A[v]);
       b[slot][c * V + v] = B[v];
     }
   }
@@ -242,261 +263,441 @@ struct SlotMaps {
   }
 };
 
+// Workgroups of the scan: kScanSlots time slots of eight lanes, which read a row's
+// 128 bytes.
 template <class T>
-constexpr int vec_of() {
-  return 16 / (int)sizeof(T);
+struct Scan {
+  static constexpr int V = 16 / (int)sizeof(T);
+  static constexpr int kLanes = 8;
+  static constexpr int kThreads = kScanSlots * kLanes;
+  static constexpr int CB = kLanes * V;
+};
+
+// ---------------------------------------------------------------------------
+// What enters a tile. Workgroups take their tiles in the order in which the
+// recurrence meets them (`l`: ascending forward, descending backward), by a
+// counter, so that a tile's workgroup only ever waits for workgroups that have
+// started before it. Each leaves its tile's map, one 64-bit word per channel that
+// says by itself whether it has been written, and the last tile of every
+// kScanGroup leaves the map of its group. What enters a tile then comes from the
+// maps of the groups before its own and of the tiles before it in its group, from
+// the tile on that holds the sequence's first token: two hops however long the
+// sequence, and the same order of sums in every run.
+// ---------------------------------------------------------------------------
+constexpr unsigned long long kNoWord = ~0ull;
+
+__device__ __forceinline__ void put_word(unsigned long long* w, float A, float B) {
+  unsigned a = __float_as_uint(A);
+  if (a == 0xffffffffu) a = 0xffc00000u;  // a NaN like the empty word's
+  __hip_atomic_store(w, (unsigned long long)__float_as_uint(B) << 32 | a, __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// Forward. PHASE 0 leaves each tile's map; PHASE 1 reads what enters each tile
-// and runs its tokens.
-template <class T, class G, int FORM, bool PACKED, int PHASE>
-__global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanArgs p, int cblocks) {
-  constexpr int V = vec_of<T>(), CB = kScanLanes * V, LT = kScanTokensFwd;
-  __shared__ SlotMaps<CB> sm;
-  const int c = threadIdx.x % kScanLanes, slot = threadIdx.x / kScanLanes;
-  const long long tile = blockIdx.x / cblocks;
-  const int cb = blockIdx.x % cblocks;
-  const int ch = cb * CB + c * V;
-  const int n = p.H - ch;
-  const Tokens<LT> k = tokens_of<LT, PACKED>(p, tile * kScanTileFwd + (long long)slot * LT);
-  Loaded<T, G, V, LT> d;
-  load_tokens<T, G, V, LT, PACKED>(p, k, ch, n, d);
-  float A[V], B[V];
+// (A, B) composed with the words w[0], w[stride], ... of n maps, in their order;
+// waits until each has been written.
+__device__ __forceinline__ void fold_words(const unsigned long long* w, long long stride, int n, float& A,
+                                           float& B) {
+  constexpr int kBatch = 8;
+  for (int i = 0; i < n; i += kBatch) {
+    unsigned long long q[kBatch];
+    bool all;
+    do {
+      all = true;
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    A[v] = 1.f;
-    B[v] = 0.f;
+      for (int j = 0; j < kBatch; ++j)
+        q[j] = i + j < n ? __hip_atomic_load(w + (i + j) * stride, __ATOMIC_RELAXED,
+                                             __HIP_MEMORY_SCOPE_AGENT)
+                         : 0;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) all = all && q[j] != kNoWord;
+      if (!all) __builtin_amdgcn_s_sleep(1);
+    } while (!all);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (i + j < n) {
+        const float a = __uint_as_float((unsigned)q[j]), b = __uint_as_float((unsigned)(q[j] >> 32));
+        B = leave(a, b, B);
+        A = drops(a) ? a : A * a;
+      }
   }
+}
+
+template <int CB, int THREADS>
+struct LookBack {
+  static constexpr int kParts = THREADS / CB;
+  float a[kParts][CB], b[kParts][CB];
+  float enter[CB];
+
+  // Leaves the tile's map (A, B: valid in threads below CB) and what enters the
+  // tile, in enter[]. `first`: the tile from which on maps count, l for none.
+  __device__ __forceinline__ void run(const ScanArgs& p, int l, int first, int c0, float A,
+                                      float B) {
+    const int c = threadIdx.x % CB, part = threadIdx.x / CB;
+    const bool in = c0 + c < p.H;
+    unsigned long long* w = p.words + c0 + c;
+    if (part == 0 && in) put_word(w + (long long)l * p.H, A, B);
+    const int g = l / kScanGroup, g0 = g * kScanGroup;
+    unsigned long long* gw = p.words + p.ntiles * p.H + c0 + c;
+    const bool last = l == g0 + kScanGroup - 1;
+    // the tiles before this one in its group; a group's map takes all of them
+    const int from = last || first < g0 ? g0 : first;
+    share(w + (long long)from * p.H, p.H, in ? l - from : 0, part, c);
+    __syncthreads();
+    float ta = 1.f, tb = 0.f;
+    if (part == 0) {
+      join(c, ta, tb);
+      if (last && in) put_word(gw + (long long)g * p.H, drops(A) ? A : ta * A, leave(A, B, tb));
+    }
+    __syncthreads();
+    const int gf = first / kScanGroup;
+    share(gw + (long long)gf * p.H, p.H, in && first < g0 ? g - gf : 0, part, c);
+    __syncthreads();
+    if (part == 0) {
+      float ga = 1.f, gb = 0.f;
+      join(c, ga, gb);
+      enter[c] = first < l ? leave(ta, tb, gb) : 0.f;
+    }
+    __syncthreads();
+  }
+
+  // This part's share of n words.
+  __device__ __forceinline__ void share(const unsigned long long* w, long long stride, int n, int part,
+                                        int c) {
+    const int per = (n + kParts - 1) / kParts, i0 = part * per;
+    float A = 1.f, B = 0.f;
+    fold_words(w + i0 * stride, stride, i0 + per < n ? per : n - i0, A, B);
+    a[part][c] = A;
+    b[part][c] = B;
+  }
+  __device__ __forceinline__ void join(int c, float& A, float& B) {
 #pragma unroll
-  for (int i = 0; i < LT; ++i) {
-    float a[V], u[V];
-    maps_of<FORM>(p, k, d, i, ch, n, a, u);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      B[v] = leave(a[v], u[v], B[v]);
-      A[v] = drops(a[v]) ? a[v] : A[v] * a[v];
+    for (int q = 0; q < kParts; ++q) {
+      B = leave(a[q][c], b[q][c], B);
+      A = drops(a[q][c]) ? a[q][c] : A * a[q][c];
     }
   }
-  sm.put(slot, c, A, B);
+};
+
+// The next tile in order and its block of channels.
+__device__ __forceinline__ unsigned take_ticket(const ScanArgs& p) {
+  __shared__ unsigned ticket;
+  if (threadIdx.x == 0)
+    ticket = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  return ticket;
+}
+
+// The compiler forgets what it has computed from r: it computes that again later,
+// and keeps only r in registers meanwhile.
+template <class T, int V, int LT>
+__device__ __forceinline__ void forget(Vec<T, V> (&r)[LT]) {
+#pragma unroll
+  for (int i = 0; i < LT; ++i)
+#pragma unroll
+    for (int j = 0; j < Vec<T, V>::kWords; ++j) asm volatile("" : "+v"(r[i].w[j]));
+}
+
+// LOOK: tiles hand states on; else every tile begins with a sequence, or is the
+// only one.
+template <class T, class G, int FORM, bool PACKED, bool LOOK>
+__global__ __launch_bounds__(Scan<T>::kThreads, 4) void scan_fwd_kernel(ScanArgs p) {
+  constexpr int V = Scan<T>::V, CB = Scan<T>::CB, LT = kScanTokens, NT = Scan<T>::kThreads;
+  __shared__ SlotMaps<CB, NT> sm;
+  __shared__ LookBack<LOOK ? CB : NT, NT> lb;
+  const int c = threadIdx.x % Scan<T>::kLanes, slot = threadIdx.x / Scan<T>::kLanes;
+  const unsigned id = LOOK ? take_ticket(p) : blockIdx.x;
+  const int tile = id / p.cblocks;
+  const int c0 = id % p.cblocks * CB, ch = c0 + c * V, n = p.H - ch;
+  const Tokens<LT> k = tokens_of<LT, PACKED>(p, tile * kScanTile + slot * LT);
+  // after token i, h = A[i] h_in + B[i], of the state that enters the slot
+  float A[LT][V], B[LT][V];
+  {
+    Vec<T, V> x[LT];
+    Vec<G, V> g[LT];
+    load_tokens<T, V, LT, PACKED>(p.x, p.sxb, p.sxt, p, k, ch, n, x);
+    load_tokens<G, V, LT, PACKED>(p.g, p.sgb, p.sgt, p, k, ch, n, g);
+    float pa[V], pb[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      pa[v] = 1.f;
+      pb[v] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < LT; ++i) {
+      if (k.start >> i & 1) {
+        begin_state<V>(p, k, i, ch, n, pb);
+#pragma unroll
+        for (int v = 0; v < V; ++v) pa[v] = 0.f;
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float a, na;
+        gate_of<FORM>(g[i].get(v), a, na);
+        const float xv = x[i].get(v);
+        pa[v] *= a;
+        pb[v] = fmaf(a, pb[v], FORM == LTC_GATE_BLEND ? na * xv : xv);
+        A[i][v] = pa[v];
+        B[i][v] = pb[v];
+      }
+    }
+  }
+  sm.put(slot, c, A[LT - 1], B[LT - 1], k.start != 0);
   __syncthreads();
   sm.compose();
   __syncthreads();
-  if constexpr (PHASE == 0) {
-    const int cc = threadIdx.x;
-    if (cc < CB && cb * CB + cc < p.H) {
-      float ta, tb;
-      sm.whole(cc, ta, tb);
-      p.agg_a[tile * p.H + cb * CB + cc] = ta;
-      p.agg_b[tile * p.H + cb * CB + cc] = tb;
+  if constexpr (LOOK) {
+    // the tile of the first token's sequence's beginning
+    const int t0 = tile * kScanTile;
+    int first = tile;
+    if constexpr (PACKED) {
+      const int m = p.marks[t0];
+      if (m >= 0 && !(m & kMarkStart)) first = begin_of(p, m >> 2, t0) / kScanTile;
+    } else {
+      const int q = t0 - (int)((unsigned)t0 % (unsigned)p.T);
+      if (q < t0) first = q / kScanTile;
     }
-  } else {
-    if (n <= 0) return;
-    Vec<float, V> h{};
-    if (tile > 0) h = load_vec<float, V>(p.carry + tile * p.H + ch, n);
-#pragma unroll
-    for (int v = 0; v < V; ++v) h.v[v] = sm.enter(slot, c * V + v, h.v[v]);
-    if (p.states != nullptr && k.t0 % kScanTileBwd == 0 && k.t0 < p.N)
-      store_vec<float, V>(p.states + k.t0 / kScanTileBwd * p.H + ch, h, n);
-#pragma unroll
-    for (int i = 0; i < LT; ++i) {
-      if (k.t0 + i >= p.N) break;
-      float a[V], u[V];
-      maps_of<FORM>(p, k, d, i, ch, n, a, u);
-      Vec<T, V> o;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        h.v[v] = leave(a[v], u[v], h.v[v]);
-        o.v[v] = (T)h.v[v];
-      }
-      store_vec<T, V>(static_cast<T*>(p.out) + (k.t0 + i) * p.H + ch, o, n);
-      if (k.end >> i & 1) store_vec<float, V>(p.hf + (long long)k.b[i] * p.H + ch, h, n);
-    }
+    float ta = 1.f, tb = 0.f;
+    if (threadIdx.x < CB) sm.whole(threadIdx.x, ta, tb);
+    lb.run(p, tile, first, c0, ta, tb);
   }
-}
-
-// What enters every tile, one thread per channel; REV for the backward's order.
-template <bool REV>
-__global__ __launch_bounds__(64) void scan_carry_kernel(ScanArgs p, long long ntiles) {
-  const int ch = blockIdx.x * 64 + threadIdx.x;
-  if (ch >= p.H) return;
-  float h = 0.f;
-  for (long long j = 0; j < ntiles; ++j) {
-    const long long at = (REV ? ntiles - 1 - j : j) * p.H + ch;
-    p.carry[at] = h;
-    h = leave(p.agg_a[at], p.agg_b[at], h);
+  if (n <= 0) return;
+  float h[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) h[v] = sm.enter(slot, c * V + v, LOOK ? lb.enter[c * V + v] : 0.f);
+  // the backward starts its tiles from these
+  if (p.states != nullptr && slot == 0) {
+    Vec<float, V> q;
+    q.put(h);
+    store_vec<float, V>(p.states + (long long)tile * p.H + ch, q, n);
+  }
+  T* out = static_cast<T*>(p.out) + (long long)k.t0 * p.H + ch;
+#pragma unroll
+  for (int i = 0; i < LT; ++i) {
+    if (k.t0 + i >= p.N) break;
+    if (k.start >> i & 1) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[v] = 0.f;  // A[i] is 0 from here on
+    }
+    float o[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) o[v] = fmaf(A[i][v], h[v], B[i][v]);
+    Vec<T, V> q;
+    q.put(o);
+    store_vec<T, V>(out, q, n);
+    out += p.H;
+    if (k.end >> i & 1) {
+      Vec<float, V> f;
+      f.put(o);
+      store_vec<float, V>(p.hf + (long long)k.b[i] * p.H + ch, f, n);
+    }
   }
 }
 
 // Backward: the carry from token t + 1 to t is a_{t+1} d_{t+1}, nothing across
-// sequences.
-template <class T, class G, int FORM, bool PACKED, int PHASE>
-__global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs p, int cblocks) {
-  constexpr int V = vec_of<T>(), CB = kScanLanes * V, LT = kScanTokensBwd;
-  __shared__ SlotMaps<CB> sf, sr;
-  const int c = threadIdx.x % kScanLanes, slot = threadIdx.x / kScanLanes;
-  const long long tile = blockIdx.x / cblocks;
-  const int cb = blockIdx.x % cblocks;
-  const int ch = cb * CB + c * V;
-  const int n = p.H - ch;
-  const Tokens<LT> k = tokens_of<LT, PACKED>(p, tile * kScanTileBwd + (long long)slot * LT);
-  Loaded<T, G, V, LT> d;
-  load_tokens<T, G, V, LT, PACKED>(p, k, ch, n, d);
-  // dL/dout, with dL/d state_final at a sequence's last token
-  Vec<T, V> go[LT];
+// sequences. The states are run again from what entered the tile.
+template <class T, class G, int FORM, bool PACKED, bool LOOK>
+__global__ __launch_bounds__(Scan<T>::kThreads, 3) void scan_bwd_kernel(ScanArgs p) {
+  constexpr int V = Scan<T>::V, CB = Scan<T>::CB, LT = kScanTokens, NT = Scan<T>::kThreads;
+  __shared__ SlotMaps<CB, NT> sf, sr;
+  __shared__ LookBack<LOOK ? CB : NT, NT> lb;
+  const int c = threadIdx.x % Scan<T>::kLanes, slot = threadIdx.x / Scan<T>::kLanes;
+  const unsigned id = LOOK ? take_ticket(p) : blockIdx.x;
+  const int l = id / p.cblocks, tile = (int)p.ntiles - 1 - l;
+  const int c0 = id % p.cblocks * CB, ch = c0 + c * V, n = p.H - ch;
+  const Tokens<LT> k = tokens_of<LT, PACKED>(p, tile * kScanTile + slot * LT);
+  Vec<T, V> x[LT], go[LT];
+  Vec<G, V> g[LT];
+  load_tokens<T, V, LT, PACKED>(p.x, p.sxb, p.sxt, p, k, ch, n, x);
+  load_tokens<G, V, LT, PACKED>(p.g, p.sgb, p.sgt, p, k, ch, n, g);
+  load_tokens<T, V, LT, PACKED>(p.go, p.sob, p.sot, p, k, ch, n, go);
+  // o += dL/d state_final, at a sequence's last token
+  auto add_end = [&](int i, float(&o)[V]) {
+    if (p.gh == nullptr || n <= 0 || !(k.end >> i & 1)) return;
+    const Vec<float, V> gh = load_vec<float, V>(p.gh + (long long)k.b[i] * p.H + ch, n);
 #pragma unroll
-  for (int i = 0; i < LT; ++i) {
-    go[i] = Vec<T, V>{};
-    if (p.go != nullptr && n > 0 && (k.valid >> i & 1))
-      go[i] = load_vec<T, V>(static_cast<const T*>(p.go) + row_of<PACKED>(k, i, p.sob, p.sot) + ch, n);
-  }
-  auto grad_at = [&](int i, float(&o)[V]) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) o[v] = (float)go[i].v[v];
-    if (p.gh != nullptr && n > 0 && (k.end >> i & 1)) {
-      const Vec<float, V> gh = load_vec<float, V>(p.gh + (long long)k.b[i] * p.H + ch, n);
-#pragma unroll
-      for (int v = 0; v < V; ++v) o[v] += gh.v[v];
-    }
+    for (int v = 0; v < V; ++v) o[v] += gh.get(v);
   };
-  float A[V], B[V], C[V], D[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    A[v] = C[v] = 1.f;
-    B[v] = D[v] = 0.f;
-  }
-#pragma unroll
-  for (int i = 0; i < LT; ++i) {
-    float a[V], u[V];
-    maps_of<FORM>(p, k, d, i, ch, n, a, u);
+  {
+    // the map of the slot's tokens, and of the carries through them
+    float a[LT][V], A[V], B[V], D[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      B[v] = leave(a[v], u[v], B[v]);
-      A[v] = drops(a[v]) ? a[v] : A[v] * a[v];
-    }
-  }
-#pragma unroll
-  for (int i = LT - 1; i >= 0; --i) {
-    float a[V], u[V], o[V];
-    maps_of<FORM>(p, k, d, i, ch, n, a, u);
-    grad_at(i, o);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      // nothing passes to the token before a sequence's first
-      D[v] = drops(a[v]) ? 0.f : a[v] * (o[v] + D[v]);
-      C[v] = drops(a[v]) ? a[v] : C[v] * a[v];
-    }
-  }
-  if constexpr (PHASE == 1) sf.put(slot, c, A, B);
-  sr.put(kScanSlots - 1 - slot, c, C, D);
-  __syncthreads();
-  if constexpr (PHASE == 1) sf.compose();
-  sr.compose();
-  __syncthreads();
-  if constexpr (PHASE == 0) {
-    const int cc = threadIdx.x;
-    if (cc < CB && cb * CB + cc < p.H) {
-      float ta, tb;
-      sr.whole(cc, ta, tb);
-      p.agg_a[tile * p.H + cb * CB + cc] = ta;
-      p.agg_b[tile * p.H + cb * CB + cc] = tb;
-    }
-  } else {
-    if (n <= 0 || k.t0 >= p.N) return;
-    Vec<float, V> h = load_vec<float, V>(p.states + tile * p.H + ch, n);
-    Vec<float, V> e = load_vec<float, V>(p.carry + tile * p.H + ch, n);
-    float hp[LT][V];  // state before token i
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      hp[0][v] = sf.enter(slot, c * V + v, h.v[v]);
-      e.v[v] = sr.enter(kScanSlots - 1 - slot, c * V + v, e.v[v]);
+      A[v] = 1.f;
+      B[v] = D[v] = 0.f;
     }
 #pragma unroll
-    for (int i = 0; i + 1 < LT; ++i) {
-      float a[V], u[V];
-      maps_of<FORM>(p, k, d, i, ch, n, a, u);
+    for (int i = 0; i < LT; ++i) {
+      if (k.start >> i & 1) begin_state<V>(p, k, i, ch, n, B);
 #pragma unroll
-      for (int v = 0; v < V; ++v) hp[i + 1][v] = leave(a[v], u[v], hp[i][v]);
+      for (int v = 0; v < V; ++v) {
+        float na;
+        gate_of<FORM>(g[i].get(v), a[i][v], na);
+        const float xv = x[i].get(v);
+        A[v] *= a[i][v];
+        B[v] = fmaf(a[i][v], B[v], FORM == LTC_GATE_BLEND ? na * xv : xv);
+      }
     }
 #pragma unroll
     for (int i = LT - 1; i >= 0; --i) {
-      if (k.t0 + i >= p.N) continue;
-      const bool valid = k.valid >> i & 1, start = k.start >> i & 1;
       float o[V];
-      grad_at(i, o);
-      Vec<float, V> h0 = start ? state_of<V>(p, k, i, ch, n) : Vec<float, V>{};
-      Vec<T, V> gx;
-      Vec<G, V> gg;
-      Vec<float, V> gs;
+#pragma unroll
+      for (int v = 0; v < V; ++v) o[v] = go[i].get(v);
+      add_end(i, o);
+#pragma unroll
+      for (int v = 0; v < V; ++v) D[v] = a[i][v] * (o[v] + D[v]);
+      if (k.start >> i & 1) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) D[v] = 0.f;
+      }
+    }
+    sf.put(slot, c, A, B, k.start != 0);
+    sr.put(kScanSlots - 1 - slot, c, A, D, k.start != 0);
+  }
+  __syncthreads();
+  sf.compose();
+  sr.compose();
+  __syncthreads();
+  if constexpr (LOOK) {
+    // the tile of the end of the last token's sequence
+    const int t1 = tile * kScanTile + kScanTile - 1 < p.N ? tile * kScanTile + kScanTile - 1 : (int)p.N - 1;
+    int first = l;
+    if constexpr (PACKED) {
+      const int m = p.marks[t1];
+      if (m >= 0 && !(m & kMarkEnd)) first = (int)p.ntiles - 1 - end_of(p, m >> 2, t1) / kScanTile;
+    } else {
+      const int q = t1 - (int)((unsigned)t1 % (unsigned)p.T) + p.T - 1;
+      if (q > t1) first = (int)p.ntiles - 1 - q / kScanTile;
+    }
+    float ta = 1.f, tb = 0.f;
+    if (threadIdx.x < CB) sr.whole(threadIdx.x, ta, tb);
+    lb.run(p, l, first, c0, ta, tb);
+  }
+  forget(x);
+  forget(g);
+  forget(go);
+  if (n <= 0 || k.t0 >= p.N) return;
+  float hp[LT][V], na[LT][V], a[LT][V], e[V];  // state before token i, carry into it
+  {
+    const Vec<float, V> q = load_vec<float, V>(p.states + (long long)tile * p.H + ch, n);
+    float h[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      h[v] = sf.enter(slot, c * V + v, q.get(v));
+      e[v] = sr.enter(kScanSlots - 1 - slot, c * V + v, LOOK ? lb.enter[c * V + v] : 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < LT; ++i) {
+      if (k.start >> i & 1) begin_state<V>(p, k, i, ch, n, h);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        float a, na;
-        gate_of<FORM>((float)d.g[i].v[v], a, na);
-        const float x = (float)d.x[i].v[v], hb = start ? h0.v[v] : hp[i][v];
-        const float dt = valid ? o[v] + e.v[v] : 0.f;
-        gx.v[v] = (T)(na * dt);
-        if constexpr (FORM == LTC_GATE_BLEND) gg.v[v] = (G)(valid ? dt * (hb - x) * (a * na) : 0.f);
-        else gg.v[v] = (G)(valid ? dt * hb * a : 0.f);
-        gs.v[v] = a * dt;
-        e.v[v] = start || !valid ? 0.f : gs.v[v];
+        gate_of<FORM>(g[i].get(v), a[i][v], na[i][v]);
+        const float xv = x[i].get(v);
+        hp[i][v] = h[v];
+        h[v] = fmaf(a[i][v], h[v], FORM == LTC_GATE_BLEND ? na[i][v] * xv : xv);
       }
-      const long long at = (k.t0 + i) * p.H + ch;
-      if (p.gx != nullptr) store_vec<T, V>(static_cast<T*>(p.gx) + at, gx, n);
-      if (p.gg != nullptr) store_vec<G, V>(static_cast<G*>(p.gg) + at, gg, n);
-      if (start && p.gs != nullptr) store_vec<float, V>(p.gs + (long long)k.b[i] * p.H + ch, gs, n);
+    }
+  }
+  long long at = (long long)k.t0 * p.H + ch + (LT - 1) * (long long)p.H;
+#pragma unroll
+  for (int i = LT - 1; i >= 0; --i, at -= p.H) {
+    if (k.t0 + i >= p.N) continue;
+    float o[V], dx[V], dg[V], ds[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) o[v] = go[i].get(v);
+    add_end(i, o);
+    if (!(k.valid >> i & 1)) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) e[v] = hp[i][v] = 0.f;
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float d = o[v] + e[v];
+      e[v] = ds[v] = a[i][v] * d;
+      if constexpr (FORM == LTC_GATE_BLEND) {
+        dx[v] = na[i][v] * d;
+        dg[v] = ds[v] * (na[i][v] * (hp[i][v] - x[i].get(v)));
+      } else {
+        dx[v] = d;
+        dg[v] = ds[v] * hp[i][v];
+      }
+    }
+    if (p.gx != nullptr) {
+      Vec<T, V> q;
+      q.put(dx);
+      store_vec<T, V>(static_cast<T*>(p.gx) + at, q, n);
+    }
+    if (p.gg != nullptr) {
+      Vec<G, V> q;
+      q.put(dg);
+      store_vec<G, V>(static_cast<G*>(p.gg) + at, q, n);
+    }
+    if (k.start >> i & 1) {
+      if (p.gs != nullptr && (k.valid >> i & 1)) {
+        Vec<float, V> q;
+        q.put(ds);
+        store_vec<float, V>(p.gs + (long long)k.b[i] * p.H + ch, q, n);
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) e[v] = 0.f;
     }
   }
 }
 
-// The mark of every packed token: the last sequence that starts at or before
-// it, by bisection. Any boundaries give marks in range; those of ascending
-// boundaries are right.
-__global__ __launch_bounds__(256) void scan_marks_kernel(const int* cu, int S, long long N, int* marks) {
-  const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (t >= N) return;
-  int lo = 0, hi = S + 1;  // first index whose boundary lies behind t
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (cu[mid] <= t) lo = mid + 1;
-    else hi = mid;
-  }
-  const int s = lo - 1;
-  int m = kMarkNone;
-  if (s >= 0 && s < S)
-    m = 4 * s + (cu[s] == t ? kMarkStart : 0) + (cu[s + 1] == t + 1 || t + 1 == N ? kMarkEnd : 0);
-  marks[t] = m;
+// Before the scan: no words, the first ticket; for packed tokens their marks (the
+// last sequence that starts at or before a token, by bisection: any boundaries
+// give marks in range, ascending ones the right ones), and dst = src for the
+// empty sequences, which no token writes (all of them without tokens).
+__global__ __launch_bounds__(256) void scan_prep_kernel(ScanPrep p) {
+  const long long i0 = (long long)blockIdx.x * 256 + threadIdx.x, step = (long long)gridDim.x * 256;
+  for (long long i = i0; i < p.nwords; i += step) p.words[i] = kNoWord;
+  if (i0 == 0 && p.ticket != nullptr) *p.ticket = 0;
+  if (p.marks != nullptr)
+    for (long long t = i0; t < p.N; t += step) {
+      int lo = 0, hi = p.S + 1;  // first index whose boundary lies behind t
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (p.cu[mid] <= t) lo = mid + 1;
+        else hi = mid;
+      }
+      const int s = lo - 1;
+      int m = kMarkNone;
+      if (s >= 0 && s < p.S)
+        m = 4 * s + (p.cu[s] == t ? kMarkStart : 0) + (p.cu[s + 1] == t + 1 || t + 1 == p.N ? kMarkEnd : 0);
+      p.marks[t] = m;
+    }
+  if (p.dst != nullptr)
+    for (long long i = i0; i < (long long)p.S * p.H; i += step) {
+      const int s = (int)(i / p.H);
+      // a sequence that begins outside the tokens has none either
+      const bool empty = p.N == 0 || p.cu[s + 1] <= p.cu[s] || p.cu[s] >= p.N || p.cu[s] < 0;
+      if (empty) p.dst[i] = p.src != nullptr ? p.src[i] : 0.f;
+    }
 }
 
-__global__ __launch_bounds__(256) void scan_empty_kernel(const int* cu, int S, int H, long long N,
-                                                         const float* src, float* dst) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (long long)S * H) return;
-  const int s = (int)(i / H);
-  // a sequence whose first token lies behind the tokens has none either
-  const bool empty = cu == nullptr || cu[s + 1] <= cu[s] || cu[s] >= N || cu[s] < 0;
-  if (empty) dst[i] = src != nullptr ? src[i] : 0.f;
-}
+constexpr int kStepThreads = 256, kStepChannels = 4;
 
 // One token of each row, its state updated in place. A row whose slot an
 // earlier row names too is left to that row, which takes the rows of its slot
 // one after the other, as tokens of one stream.
 template <class T, class G, int FORM>
-__global__ __launch_bounds__(kScanThreads) void scan_step_kernel(StepArgs p) {
-  constexpr int V = vec_of<T>();
+__global__ __launch_bounds__(kStepThreads) void scan_step_kernel(StepArgs p) {
+  constexpr int V = kStepChannels;
   const int row = blockIdx.y;
-  const int ch = (blockIdx.x * kScanThreads + threadIdx.x) * V;
+  const int ch = (blockIdx.x * kStepThreads + threadIdx.x) * V;
   const int n = p.H - ch;
   int slot = row;
   if (p.slots != nullptr) {
     slot = p.slots[row];
     int earlier = 0;
-    for (int r = threadIdx.x; r < row; r += kScanThreads) earlier |= p.slots[r] == slot;
+    for (int r = threadIdx.x; r < row; r += kStepThreads) earlier |= p.slots[r] == slot;
     const bool live = slot >= 0 && slot < p.P;
     if (!live) {
       // padding gives zeros, a slot that is not there NaN
-      const float f = slot < 0 ? 0.f : __builtin_nanf("");
-      Vec<T, V> o;
+      float f[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) o.v[v] = (T)f;
+      for (int v = 0; v < V; ++v) f[v] = slot < 0 ? 0.f : __builtin_nanf("");
+      Vec<T, V> o;
+      o.put(f);
       if (n > 0) store_vec<T, V>(static_cast<T*>(p.out) + (long long)row * p.H + ch, o, n);
     }
     if (__syncthreads_or(earlier) || !live) return;
@@ -511,20 +712,21 @@ __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(StepArgs p) {
     }
     const Vec<T, V> x = load_vec<T, V>(static_cast<const T*>(p.x) + r * p.sxb + ch, n);
     const Vec<G, V> g = load_vec<G, V>(static_cast<const G*>(p.g) + r * p.sgb + ch, n);
-    Vec<T, V> o;
+    float f[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       float a, na;
-      gate_of<FORM>((float)g.v[v], a, na);
-      h.v[v] = fmaf(a, h.v[v], na * (float)x.v[v]);
-      o.v[v] = (T)h.v[v];
+      gate_of<FORM>(g.get(v), a, na);
+      f[v] = fmaf(a, h.get(v), na * x.get(v));
     }
+    h.put(f);
+    Vec<T, V> o;
+    o.put(f);
     store_vec<T, V>(static_cast<T*>(p.out) + (long long)r * p.H + ch, o, n);
   }
   store_vec<float, V>(sp, h, n);
 }
 
-int x_vec(int x_type) { return x_type == LTC_F32 ? 4 : 8; }
 
 // Calls f with the element types of x and the gate.
 template <class F>
@@ -547,69 +749,52 @@ hipError_t with_form(int form, bool packed, F&& f) {
 
 }  // namespace
 
-ScanPlan scan_plan(int x_type, int g_type, int form, bool packed, long long N, int H, bool bwd) {
-  ScanPlan p{};
-  p.x_type = x_type;
-  p.g_type = g_type;
-  p.form = form;
-  p.packed = packed;
-  p.tile = bwd ? kScanTileBwd : kScanTileFwd;
-  p.ntiles = (N + p.tile - 1) / p.tile;
-  const int cb = kScanLanes * x_vec(x_type);
-  p.cblocks = (H + cb - 1) / cb;
-  return p;
+void scan_tiles(int x_type, long long N, int H, long long* ntiles, int* cblocks) {
+  const int cb = x_type == LTC_F32 ? Scan<float>::CB : Scan<__bf16>::CB;
+  *ntiles = (N + kScanTile - 1) / kScanTile;
+  *cblocks = (H + cb - 1) / cb;
 }
 
-hipError_t launch_scan_marks(const int* cu, int S, long long N, int* marks, hipStream_t s) {
-  LTC_LAUNCH(scan_marks_kernel, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, s, cu, S, N, marks);
+// Whether states pass from tile to tile.
+bool scan_looks(long long N, int T, bool packed) {
+  return N > kScanTile && (packed || kScanTile % T != 0);
+}
+
+hipError_t launch_scan_prep(const ScanPrep& p, hipStream_t s) {
+  long long n = p.nwords;
+  if (p.marks != nullptr && p.N > n) n = p.N;
+  if (p.dst != nullptr && (long long)p.S * p.H > n) n = (long long)p.S * p.H;
+  const long long blocks = (n + 255) / 256;
+  LTC_LAUNCH(scan_prep_kernel, dim3((unsigned)(blocks < 1 ? 1 : blocks > 2048 ? 2048 : blocks)), dim3(256),
+             0, s, p);
   return hipGetLastError();
 }
 
-hipError_t launch_scan_empty(const int* cu, int S, int H, long long N, const float* src, float* dst,
-                             hipStream_t s) {
-  const long long n = (long long)S * H;
-  LTC_LAUNCH(scan_empty_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, cu, S, H, N, src,
-             dst);
-  return hipGetLastError();
-}
-
-hipError_t launch_scan_fwd(const ScanPlan& p, const ScanArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)(p.ntiles * p.cblocks)), block(kScanThreads);
-  return with_types(p.x_type, p.g_type, [&](auto t, auto g) {
-    return with_form(p.form, p.packed, [&](auto form, auto packed) {
+hipError_t launch_scan(const ScanTypes& ty, const ScanArgs& a, bool bwd, hipStream_t s) {
+  const dim3 grid((unsigned)(a.ntiles * a.cblocks));
+  const bool look = scan_looks(a.N, a.T, a.marks != nullptr);
+  return with_types(ty.x, ty.g, [&](auto t, auto g) {
+    return with_form(ty.form, a.marks != nullptr, [&](auto form, auto packed) {
       using T = decltype(t);
       using G = decltype(g);
+      const dim3 block(Scan<T>::kThreads);
       constexpr int F = decltype(form)::value;
       constexpr bool P = decltype(packed)::value;
-      if (p.ntiles > 1) {
-        LTC_LAUNCH((scan_fwd_kernel<T, G, F, P, 0>), grid, block, 0, s, a, p.cblocks);
-        LTC_LAUNCH(scan_carry_kernel<false>, dim3((a.H + 63) / 64), dim3(64), 0, s, a, p.ntiles);
+      if (bwd) {
+        if (look) LTC_LAUNCH((scan_bwd_kernel<T, G, F, P, true>), grid, block, 0, s, a);
+        else LTC_LAUNCH((scan_bwd_kernel<T, G, F, P, false>), grid, block, 0, s, a);
+      } else {
+        if (look) LTC_LAUNCH((scan_fwd_kernel<T, G, F, P, true>), grid, block, 0, s, a);
+        else LTC_LAUNCH((scan_fwd_kernel<T, G, F, P, false>), grid, block, 0, s, a);
       }
-      LTC_LAUNCH((scan_fwd_kernel<T, G, F, P, 1>), grid, block, 0, s, a, p.cblocks);
-      return hipGetLastError();
-    });
-  });
-}
-
-hipError_t launch_scan_bwd(const ScanPlan& p, const ScanArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)(p.ntiles * p.cblocks)), block(kScanThreads);
-  return with_types(p.x_type, p.g_type, [&](auto t, auto g) {
-    return with_form(p.form, p.packed, [&](auto form, auto packed) {
-      using T = decltype(t);
-      using G = decltype(g);
-      constexpr int F = decltype(form)::value;
-      constexpr bool P = decltype(packed)::value;
-      LTC_LAUNCH((scan_bwd_kernel<T, G, F, P, 0>), grid, block, 0, s, a, p.cblocks);
-      LTC_LAUNCH(scan_carry_kernel<true>, dim3((a.H + 63) / 64), dim3(64), 0, s, a, p.ntiles);
-      LTC_LAUNCH((scan_bwd_kernel<T, G, F, P, 1>), grid, block, 0, s, a, p.cblocks);
       return hipGetLastError();
     });
   });
 }
 
 hipError_t launch_scan_step(int x_type, int g_type, int form, const StepArgs& a, hipStream_t s) {
-  const int per = kScanThreads * x_vec(x_type);
-  const dim3 grid((unsigned)((a.H + per - 1) / per), (unsigned)a.B), block(kScanThreads);
+  const int per = kStepThreads * kStepChannels;
+  const dim3 grid((unsigned)((a.H + per - 1) / per), (unsigned)a.B), block(kStepThreads);
   return with_types(x_type, g_type, [&](auto t, auto g) {
     using T = decltype(t);
     using G = decltype(g);

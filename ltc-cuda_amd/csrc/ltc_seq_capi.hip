@@ -15,8 +15,8 @@ using ltc::host_timed;
 
 namespace {
 
-// Workgroups of one launch: the runtime counts threads in 32 bits.
-constexpr long long kMaxGroups = (1LL << 32) / 256 - 1;
+// Workgroups of one launch: the runtime counts threads, up to 512 each, in 32 bits.
+constexpr long long kMaxGroups = (1LL << 32) / 512 - 1;
 
 // Pieces of a workspace or of the saved buffer, each on 256 bytes; base null:
 // sizes only.
@@ -55,11 +55,16 @@ int check_scan(int B, int T, int H, int packed) {
   // sequence numbers share a word with two flags
   if (B > INT_MAX / 4 - 1) return host_fail(LTC_EUNSUPPORTED, "too many sequences");
   const long long N = tokens_in_all(B, T, packed);
-  const ltc::ScanPlan p = ltc::scan_plan(LTC_F32, LTC_F32, 0, packed != 0, N, H, true);
-  if (p.ntiles > kMaxGroups / p.cblocks || (long long)B > kMaxGroups * 256 / H)
+  long long ntiles;
+  int cblocks;
+  ltc::scan_tiles(LTC_F32, N, H, &ntiles, &cblocks);  // the type with the most blocks
+  // token numbers are 32-bit, up to a tile behind the last
+  if (N > INT_MAX - 2 * ltc::kScanTile || ntiles > kMaxGroups / cblocks || (long long)B > kMaxGroups * 256 / H)
     return host_fail(LTC_EUNSUPPORTED, "problem too large");
   return LTC_OK;
 }
+
+long long tiles_of(long long N) { return (N + ltc::kScanTile - 1) / ltc::kScanTile; }
 
 struct ScanSaved {
   float* states;
@@ -67,23 +72,25 @@ struct ScanSaved {
 };
 ScanSaved carve_saved(Pieces& c, long long N, int H, int packed) {
   ScanSaved s{};
-  s.states = c.take<float>((N + ltc::kScanTileBwd - 1) / ltc::kScanTileBwd * H);
+  s.states = c.take<float>(tiles_of(N) * H);
   s.marks = packed ? c.take<int>(N) : nullptr;
   return s;
 }
 
 struct ScanWs {
-  float *agg_a, *agg_b, *carry;
+  unsigned long long* words;
+  long long nwords;
+  unsigned* ticket;
   int* marks;
 };
-ScanWs carve_ws(Pieces& c, long long N, int H, int packed, bool bwd) {
+ScanWs carve_ws(Pieces& c, long long N, int T, int H, int packed, bool bwd) {
   ScanWs w{};
-  const int tile = bwd ? ltc::kScanTileBwd : ltc::kScanTileFwd;
-  const long long n = (N + tile - 1) / tile * H;
-  w.agg_a = c.take<float>(n);
-  w.agg_b = c.take<float>(n);
-  w.carry = c.take<float>(n);
   if (packed && !bwd) w.marks = c.take<int>(N);
+  if (N > 0 && ltc::scan_looks(N, T, packed != 0)) {
+    w.nwords = (tiles_of(N) + tiles_of(N) / ltc::kScanGroup) * H;
+    w.words = c.take<unsigned long long>(w.nwords);
+    w.ticket = c.take<unsigned>(1);
+  }
   return w;
 }
 
@@ -188,14 +195,14 @@ long long ltc_gated_scan_saved_floats(int B, int T, int H, int packed) {
 long long ltc_gated_scan_fwd_workspace_bytes(int B, int T, int H, int packed) {
   if (check_scan(B, T, H, packed) != LTC_OK) return -1;
   Pieces c{nullptr};
-  carve_ws(c, tokens_in_all(B, T, packed), H, packed, false);
+  carve_ws(c, tokens_in_all(B, T, packed), T, H, packed, false);
   return c.off;
 }
 
 long long ltc_gated_scan_bwd_workspace_bytes(int B, int T, int H, int packed) {
   if (check_scan(B, T, H, packed) != LTC_OK) return -1;
   Pieces c{nullptr};
-  carve_ws(c, tokens_in_all(B, T, packed), H, packed, true);
+  carve_ws(c, tokens_in_all(B, T, packed), T, H, packed, true);
   return c.off;
 }
 
@@ -213,12 +220,12 @@ int ltc_gated_scan_forward(const void* x, long long sxb, long long sxt, const vo
   if (B > 0 && !state_final) return host_fail(LTC_EINVAL, "state_final pointer is NULL");
   if (save && N > 0 && !saved) return host_fail(LTC_EINVAL, "save set without a saved buffer");
   Pieces need{nullptr};
-  carve_ws(need, N, H, packed, false);
+  carve_ws(need, N, T, H, packed, false);
   rc = check_workspace(need.off, workspace, workspace_bytes);
   if (rc != LTC_OK) return rc;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   Pieces cw{static_cast<char*>(workspace)}, cs{reinterpret_cast<char*>(saved)};
-  const ScanWs w = carve_ws(cw, N, H, packed, false);
+  const ScanWs w = carve_ws(cw, N, T, H, packed, false);
   ScanSaved sv{};
   if (save) sv = carve_saved(cs, N, H, packed);
   ltc::ScanArgs a{};
@@ -236,17 +243,19 @@ int ltc_gated_scan_forward(const void* x, long long sxb, long long sxt, const vo
   a.out = out;
   a.hf = state_final;
   a.states = sv.states;
-  a.agg_a = w.agg_a;
-  a.agg_b = w.agg_b;
-  a.carry = w.carry;
+  a.words = w.words;
+  a.ticket = w.ticket;
+  ltc::scan_tiles(x_type, N, H, &a.ntiles, &a.cblocks);
   int* marks = save ? sv.marks : w.marks;
+  a.cu = cu_seqlens;
   a.marks = marks;
-  const ltc::ScanPlan p = ltc::scan_plan(x_type, gate_type, form, packed != 0, N, H, false);
+  const bool ends = B > 0 && (packed || N == 0);
+  const ltc::ScanPrep pr{w.words, w.nwords, w.ticket, cu_seqlens, marks, B, H, N, state,
+                         ends ? state_final : nullptr};
   const hipError_t e = host_timed(ltc::K_SCAN_FWD, [&] {
     hipError_t e = hipSuccess;
-    if (B > 0 && (packed || N == 0)) e = ltc::launch_scan_empty(cu_seqlens, B, H, N, state, state_final, s);
-    if (e == hipSuccess && N > 0 && packed) e = ltc::launch_scan_marks(cu_seqlens, B, N, marks, s);
-    if (e == hipSuccess && N > 0) e = ltc::launch_scan_fwd(p, a, s);
+    if (w.nwords > 0 || ends || (packed && N > 0)) e = ltc::launch_scan_prep(pr, s);
+    if (e == hipSuccess && N > 0) e = ltc::launch_scan({x_type, gate_type, form}, a, false, s);
     return e;
   });
   return e == hipSuccess ? LTC_OK : host_hip_fail("gated scan launch", e);
@@ -265,13 +274,13 @@ int ltc_gated_scan_backward(const void* x, long long sxb, long long sxt, const v
   const long long N = tokens_in_all(B, T, packed);
   if (N > 0 && !saved) return host_fail(LTC_EINVAL, "saved pointer is NULL");
   Pieces need{nullptr};
-  carve_ws(need, N, H, packed, true);
+  carve_ws(need, N, T, H, packed, true);
   rc = check_workspace(need.off, workspace, workspace_bytes);
   if (rc != LTC_OK) return rc;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   Pieces cw{static_cast<char*>(workspace)};
   Pieces cs{reinterpret_cast<char*>(const_cast<float*>(saved))};
-  const ScanWs w = carve_ws(cw, N, H, packed, true);
+  const ScanWs w = carve_ws(cw, N, T, H, packed, true);
   const ScanSaved sv = carve_saved(cs, N, H, packed);
   ltc::ScanArgs a{};
   a.x = x;
@@ -285,24 +294,26 @@ int ltc_gated_scan_backward(const void* x, long long sxb, long long sxt, const v
   a.sot = sot;
   a.h0 = state;
   a.gh = grad_state_final;
+  a.cu = cu_seqlens;
   a.marks = sv.marks;
   a.B = B;
   a.T = T;
   a.H = H;
   a.N = N;
   a.states = sv.states;
-  a.agg_a = w.agg_a;
-  a.agg_b = w.agg_b;
-  a.carry = w.carry;
+  a.words = w.words;
+  a.ticket = w.ticket;
+  ltc::scan_tiles(x_type, N, H, &a.ntiles, &a.cblocks);
   a.gx = grad_x;
   a.gg = grad_gate;
   a.gs = grad_state;
-  const ltc::ScanPlan p = ltc::scan_plan(x_type, gate_type, form, packed != 0, N, H, true);
+  const bool ends = B > 0 && grad_state && (packed || N == 0);
+  const ltc::ScanPrep pr{w.words, w.nwords, w.ticket, cu_seqlens, nullptr, B, H, N, grad_state_final,
+                         ends ? grad_state : nullptr};
   const hipError_t e = host_timed(ltc::K_SCAN_BWD, [&] {
     hipError_t e = hipSuccess;
-    if (B > 0 && grad_state && (packed || N == 0))
-      e = ltc::launch_scan_empty(cu_seqlens, B, H, N, grad_state_final, grad_state, s);
-    if (e == hipSuccess && N > 0) e = ltc::launch_scan_bwd(p, a, s);
+    if (w.nwords > 0 || ends) e = ltc::launch_scan_prep(pr, s);
+    if (e == hipSuccess && N > 0) e = ltc::launch_scan({x_type, gate_type, form}, a, true, s);
     return e;
   });
   return e == hipSuccess ? LTC_OK : host_hip_fail("gated scan backward launch", e);

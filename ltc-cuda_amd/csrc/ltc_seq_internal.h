@@ -15,18 +15,13 @@ namespace ltc {
 // Gated linear recurrence
 // ---------------------------------------------------------------------------
 
-// Workgroups of the scan kernels: 256 threads = kScanSlots time slots of
-// kScanLanes lanes; a lane holds 16 bytes of x (V channels) of each of its
-// slot's tokens, so a slot reads rows of 128 bytes.
-constexpr int kScanThreads = 256;
-constexpr int kScanLanes = 8;
-constexpr int kScanSlots = kScanThreads / kScanLanes;
-// Consecutive tokens of a slot, forward and backward (which holds dL/dout and
-// the recomputed states too).
-constexpr int kScanTokensFwd = 8;
-constexpr int kScanTokensBwd = 4;
-constexpr int kScanTileFwd = kScanSlots * kScanTokensFwd;
-constexpr int kScanTileBwd = kScanSlots * kScanTokensBwd;
+// Time slots of a workgroup.
+constexpr int kScanSlots = 32;
+// Consecutive tokens of a slot, and tokens of a workgroup.
+constexpr int kScanTokens = 4;
+constexpr int kScanTile = kScanSlots * kScanTokens;
+// Tiles whose maps are composed into one.
+constexpr int kScanGroup = 32;
 
 struct ScanArgs {
   const void* x;
@@ -35,36 +30,42 @@ struct ScanArgs {
   long long sxb, sxt, sgb, sgt, sob, sot;  // element strides of x, gate, dL/dout
   const float* h0;   // (B,H) or null for zero
   const float* gh;   // backward: dL/d state_final (B,H) or null for zero
-  const int* marks;  // packed: one word per token, see scan_marks_kernel; else null
+  const int* cu;     // packed: boundaries (B+1); else null
+  const int* marks;  // packed: one word per token (scan_prep_kernel); else null
   int B, T, H;       // sequences, tokens of each (packed: of all), channels
   long long N;       // tokens in all
+  long long ntiles;
+  int cblocks;       // blocks of channels
   void* out;         // forward (N,H)
   float* hf;         // forward (B,H)
-  float* states;     // state before every kScanTileBwd-th token, [.][H]; forward: may be null
-  float* agg_a;      // workspace: per tile and channel the product of its decays,
-  float* agg_b;      // what it adds,
-  float* carry;      // and what enters it
+  float* states;     // what enters each tile (ntiles,H); forward: may be null
+  unsigned long long* words;  // maps of tiles (ntiles,H), then of groups of tiles
+  unsigned* ticket;
   void* gx;          // backward (N,H), or null where not wanted
   void* gg;          // backward (N,H), or null
   float* gs;         // backward (B,H), or null
 };
 
-struct ScanPlan {
-  int x_type, g_type, form;
-  bool packed;
-  int tile;          // tokens per workgroup
-  long long ntiles;
-  int cblocks;       // blocks of channels
+struct ScanTypes {
+  int x, g, form;
 };
 
-ScanPlan scan_plan(int x_type, int g_type, int form, bool packed, long long N, int H, bool bwd);
-hipError_t launch_scan_marks(const int* cu, int S, long long N, int* marks, hipStream_t s);
-// Empty sequences: dst[s] = src[s] (0 for null src) where sequence s has no
-// tokens; cu null: every sequence.
-hipError_t launch_scan_empty(const int* cu, int S, int H, long long N, const float* src, float* dst,
-                             hipStream_t s);
-hipError_t launch_scan_fwd(const ScanPlan& p, const ScanArgs& a, hipStream_t s);
-hipError_t launch_scan_bwd(const ScanPlan& p, const ScanArgs& a, hipStream_t s);
+struct ScanPrep {
+  unsigned long long* words;
+  long long nwords;
+  unsigned* ticket;
+  const int* cu;
+  int* marks;
+  int S, H;
+  long long N;
+  const float* src;
+  float* dst;
+};
+
+void scan_tiles(int x_type, long long N, int H, long long* ntiles, int* cblocks);
+bool scan_looks(long long N, int T, bool packed);
+hipError_t launch_scan_prep(const ScanPrep& p, hipStream_t s);
+hipError_t launch_scan(const ScanTypes& ty, const ScanArgs& a, bool bwd, hipStream_t s);
 
 struct StepArgs {
   const void* x;
