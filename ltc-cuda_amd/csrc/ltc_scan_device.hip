@@ -208,23 +208,41 @@ __device__ __forceinline__ void begin_state(const ScanArgs& p, const Tokens<LT>&
 __device__ __forceinline__ bool drops(float A) { return __float_as_int(A) < 0; }
 __device__ __forceinline__ float leave(float A, float B, float h) { return drops(A) ? B : fmaf(A, h, B); }
 
+// Workgroups of the scan: kScanSlots time slots of eight lanes, which read a row's
+// 128 bytes. In shared memory a lane's channels lie in places four by four, so that
+// the lanes' 16-byte accesses fill the banks: side by side, eight to a lane, they
+// met in the same banks for 27 of the forward's 100 us at B8 T4096 H2048.
+template <class T>
+struct Scan {
+  static constexpr int V = 16 / (int)sizeof(T);
+  static constexpr int kLanes = 8;
+  static constexpr int kThreads = kScanSlots * kLanes;
+  static constexpr int CB = kLanes * V;
+  static __device__ __forceinline__ int place(int lane, int v) {
+    return v / 4 * (kLanes * 4) + lane * 4 + v % 4;
+  }
+  static __device__ __forceinline__ int channel(int place) {
+    return place % (kLanes * 4) / 4 * V + place / (kLanes * 4) * 4 + place % 4;
+  }
+};
+
 // A workgroup's exchange of its slots' maps: each slot leaves the map of its
 // tokens, and every slot gets the map of all slots before it.
-template <int CB, int THREADS>
+template <class T>
 struct SlotMaps {
+  static constexpr int CB = Scan<T>::CB, THREADS = Scan<T>::kThreads, V = Scan<T>::V;
   static constexpr int kParts = THREADS / CB;  // threads per channel
   static constexpr int kPer = kScanSlots / kParts;  // slots per thread
   static_assert(kParts * CB == THREADS && kPer * kParts == kScanSlots, "slot split");
   float a[kScanSlots][CB], b[kScanSlots][CB];
   float pa[kParts][CB], pb[kParts][CB];
 
-  template <int V>
-  __device__ __forceinline__ void put(int slot, int c, const float (&A)[V], const float (&B)[V],
+  __device__ __forceinline__ void put(int slot, int lane, const float (&A)[V], const float (&B)[V],
                                       bool dropped) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      a[slot][c * V + v] = dropped ? -1.f : fabsf(A[v]);
-      b[slot][c * V + v] = B[v];
+      a[slot][Scan<T>::place(lane, v)] = dropped ? -1.f : fabsf(A[v]);
+      b[slot][Scan<T>::place(lane, v)] = B[v];
     }
   }
   // After a barrier: each slot's map is replaced by that of the slots before it
@@ -263,16 +281,6 @@ struct SlotMaps {
   }
 };
 
-// Workgroups of the scan: kScanSlots time slots of eight lanes, which read a row's
-// 128 bytes.
-template <class T>
-struct Scan {
-  static constexpr int V = 16 / (int)sizeof(T);
-  static constexpr int kLanes = 8;
-  static constexpr int kThreads = kScanSlots * kLanes;
-  static constexpr int CB = kLanes * V;
-};
-
 // ---------------------------------------------------------------------------
 // What enters a tile. Workgroups take their tiles in the order in which the
 // recurrence meets them (`l`: ascending forward, descending backward), by a
@@ -293,98 +301,148 @@ __device__ __forceinline__ void put_word(unsigned long long* w, float A, float B
                      __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// (A, B) composed with the words w[0], w[stride], ... of n maps, in their order;
-// waits until each has been written.
-__device__ __forceinline__ void fold_words(const unsigned long long* w, long long stride, int n, float& A,
-                                           float& B) {
-  constexpr int kBatch = 8;
-  for (int i = 0; i < n; i += kBatch) {
-    unsigned long long q[kBatch];
-    bool all;
-    do {
-      all = true;
+// Up to N maps' words of a channel, w[0], w[stride], ...: read at once, and again
+// until each has been written.
+template <int N>
+struct Words {
+  unsigned long long q[N];
+  // w is the same for the whole workgroup, at (in words) each thread's own.
+  __device__ __forceinline__ void read(const unsigned long long* w, unsigned at, unsigned stride, int n) {
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j)
-        q[j] = i + j < n ? __hip_atomic_load(w + (i + j) * stride, __ATOMIC_RELAXED,
-                                             __HIP_MEMORY_SCOPE_AGENT)
-                         : 0;
+    for (int j = 0; j < N; ++j)
+      q[j] = j < n ? __hip_atomic_load(w + (at + j * stride), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+  }
+  __device__ __forceinline__ bool missing() const {
+    bool m = false;
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) all = all && q[j] != kNoWord;
-      if (!all) __builtin_amdgcn_s_sleep(1);
-    } while (!all);
+    for (int j = 0; j < N; ++j) m = m || q[j] == kNoWord;
+    return m;
+  }
+  __device__ __forceinline__ void wait(const unsigned long long* w, unsigned at, unsigned stride, int n) {
+    while (missing()) {
+      __builtin_amdgcn_s_sleep(1);
+      read(w, at, stride, n);
+    }
+  }
+  // (A, B) composed with the first n, in their order.
+  __device__ __forceinline__ void fold(int n, float& A, float& B) const {
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j)
-      if (i + j < n) {
+    for (int j = 0; j < N; ++j)
+      if (j < n) {
         const float a = __uint_as_float((unsigned)q[j]), b = __uint_as_float((unsigned)(q[j] >> 32));
         B = leave(a, b, B);
         A = drops(a) ? a : A * a;
       }
   }
-}
+};
 
-template <int CB, int THREADS>
+template <class T>
 struct LookBack {
+  static constexpr int CB = Scan<T>::CB, THREADS = Scan<T>::kThreads;
   static constexpr int kParts = THREADS / CB;
-  float a[kParts][CB], b[kParts][CB];
+  static constexpr int kTiles = kScanGroup / kParts;  // a part's share of a group
+  static constexpr int kGroups = 4;  // words of a batch: more cost registers, and those spill
+  float ta[kParts][CB], tb[kParts][CB], ga[kParts][CB], gb[kParts][CB];
   float enter[CB];
 
   // Leaves the tile's map (A, B: valid in threads below CB) and what enters the
   // tile, in enter[]. `first`: the tile from which on maps count, l for none.
-  __device__ __forceinline__ void run(const ScanArgs& p, int l, int first, int c0, float A,
-                                      float B) {
+  __device__ __forceinline__ void run(const ScanArgs& p, int l, int first, int c0, float A, float B) {
     const int c = threadIdx.x % CB, part = threadIdx.x / CB;
-    const bool in = c0 + c < p.H;
-    unsigned long long* w = p.words + c0 + c;
-    if (part == 0 && in) put_word(w + (long long)l * p.H, A, B);
+    const int ch = Scan<T>::channel(c);
+    const bool in = c0 + ch < p.H;
+    const long long H = p.H;
+    unsigned long long* w = p.words + c0;
+    if (part == 0 && in) put_word(w + l * H + ch, A, B);
     const int g = l / kScanGroup, g0 = g * kScanGroup;
-    unsigned long long* gw = p.words + p.ntiles * p.H + c0 + c;
+    unsigned long long* gw = p.words + p.ntiles * H + c0;
     const bool last = l == g0 + kScanGroup - 1;
     // the tiles before this one in its group; a group's map takes all of them
     const int from = last || first < g0 ? g0 : first;
-    share(w + (long long)from * p.H, p.H, in ? l - from : 0, part, c);
-    __syncthreads();
-    float ta = 1.f, tb = 0.f;
-    if (part == 0) {
-      join(c, ta, tb);
-      if (last && in) put_word(gw + (long long)g * p.H, drops(A) ? A : ta * A, leave(A, B, tb));
-    }
-    __syncthreads();
+    const int nt = in ? l - from : 0, t0 = part * kTiles, tn = nt - t0 < kTiles ? nt - t0 : kTiles;
+    // the groups before it, each part an equal share, in batches
     const int gf = first / kScanGroup;
-    share(gw + (long long)gf * p.H, p.H, in && first < g0 ? g - gf : 0, part, c);
+    const int ng = in && first < g0 ? g - gf : 0, per = (ng + kParts - 1) / kParts, i0 = part * per;
+    const int gn = ng - i0 < per ? ng - i0 : per;
+    const unsigned long long* wt = w + from * H;
+    const unsigned long long* wg = gw + gf * H;
+    const unsigned at = (unsigned)t0 * p.H + ch, ag = (unsigned)i0 * p.H + ch;
+    Words<kTiles> qt;
+    Words<kGroups> qg;
+    qt.read(wt, at, p.H, tn);
+    qg.read(wg, ag, p.H, gn);
+    float a = 1.f, b = 0.f;
+    qt.wait(wt, at, p.H, tn);
+    qt.fold(tn, a, b);
+    ta[part][c] = a;
+    tb[part][c] = b;
+    // The group's map goes out before this tile waits for other groups': groups
+    // never wait for one another in a row.
+    if (last) {
+      __syncthreads();
+      if (part == 0 && in) {
+        a = 1.f;
+        b = 0.f;
+        join(ta, tb, c, a, b);
+        put_word(gw + g * H + ch, drops(A) ? A : a * A, leave(A, B, b));
+      }
+    }
+    a = 1.f;
+    b = 0.f;
+    qg.wait(wg, ag, p.H, gn);
+    qg.fold(gn, a, b);
+    for (int i = kGroups; i < gn; i += kGroups) {
+      const unsigned ai = ag + (unsigned)i * p.H;
+      qg.read(wg, ai, p.H, gn - i);
+      qg.wait(wg, ai, p.H, gn - i);
+      qg.fold(gn - i, a, b);
+    }
+    ga[part][c] = a;
+    gb[part][c] = b;
     __syncthreads();
     if (part == 0) {
-      float ga = 1.f, gb = 0.f;
-      join(c, ga, gb);
-      enter[c] = first < l ? leave(ta, tb, gb) : 0.f;
+      a = 1.f;
+      b = 0.f;
+      join(ga, gb, c, a, b);
+      join(ta, tb, c, a, b);
+      enter[c] = first < l ? b : 0.f;
     }
     __syncthreads();
   }
 
-  // This part's share of n words.
-  __device__ __forceinline__ void share(const unsigned long long* w, long long stride, int n, int part,
-                                        int c) {
-    const int per = (n + kParts - 1) / kParts, i0 = part * per;
-    float A = 1.f, B = 0.f;
-    fold_words(w + i0 * stride, stride, i0 + per < n ? per : n - i0, A, B);
-    a[part][c] = A;
-    b[part][c] = B;
-  }
-  __device__ __forceinline__ void join(int c, float& A, float& B) {
+  static __device__ __forceinline__ void join(const float (&pa)[kParts][CB], const float (&pb)[kParts][CB],
+                                              int c, float& A, float& B) {
 #pragma unroll
     for (int q = 0; q < kParts; ++q) {
-      B = leave(a[q][c], b[q][c], B);
-      A = drops(a[q][c]) ? a[q][c] : A * a[q][c];
+      B = leave(pa[q][c], pb[q][c], B);
+      A = drops(pa[q][c]) ? pa[q][c] : A * pa[q][c];
     }
   }
 };
 
-// The next tile in order and its block of channels.
-__device__ __forceinline__ unsigned take_ticket(const ScanArgs& p) {
-  __shared__ unsigned ticket;
-  if (threadIdx.x == 0)
-    ticket = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  return ticket;
+struct NoLookBack {};
+
+// A workgroup's tile, in order, and its block of channels. Blocks of channels are
+// dealt out in ranges of p.per, one to a workgroup number modulo p.ranges: with
+// eight ranges each is one XCD's, which then reads and writes whole stretches of a
+// row, so that lines two blocks share meet in its L2. A counter takes one addition
+// in about 15 ns, so each range has its own; one counter for all held B8 T4096
+// H2048 (8192 tiles) to 128 us, and one for each block of channels (88 where rows
+// are aligned) let neighbours drift apart: 181 us at H2047.
+template <bool LOOK>
+__device__ __forceinline__ void take_tile(const ScanArgs& p, int& tile, int& cblock) {
+  const unsigned range = blockIdx.x % p.ranges;
+  unsigned t = blockIdx.x / p.ranges;
+  if constexpr (LOOK) {
+    __shared__ unsigned ticket;
+    if (threadIdx.x == 0)
+      ticket = __hip_atomic_fetch_add(p.tickets + range * kTicketStride, 1u, __ATOMIC_RELAXED,
+                                      __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    t = ticket;
+  }
+  tile = t / p.per;
+  cblock = range * p.per + t % p.per;
 }
 
 // The compiler forgets what it has computed from r: it computes that again later,
@@ -401,13 +459,14 @@ __device__ __forceinline__ void forget(Vec<T, V> (&r)[LT]) {
 // only one.
 template <class T, class G, int FORM, bool PACKED, bool LOOK>
 __global__ __launch_bounds__(Scan<T>::kThreads, 4) void scan_fwd_kernel(ScanArgs p) {
-  constexpr int V = Scan<T>::V, CB = Scan<T>::CB, LT = kScanTokens, NT = Scan<T>::kThreads;
-  __shared__ SlotMaps<CB, NT> sm;
-  __shared__ LookBack<LOOK ? CB : NT, NT> lb;
+  constexpr int V = Scan<T>::V, CB = Scan<T>::CB, LT = kScanTokens;
+  __shared__ SlotMaps<T> sm;
+  __shared__ typename std::conditional<LOOK, LookBack<T>, NoLookBack>::type lb;
   const int c = threadIdx.x % Scan<T>::kLanes, slot = threadIdx.x / Scan<T>::kLanes;
-  const unsigned id = LOOK ? take_ticket(p) : blockIdx.x;
-  const int tile = id / p.cblocks;
-  const int c0 = id % p.cblocks * CB, ch = c0 + c * V, n = p.H - ch;
+  int tile, cblock;
+  take_tile<LOOK>(p, tile, cblock);
+  if (cblock >= p.cblocks) return;  // the last range may be short
+  const int c0 = cblock * CB, ch = c0 + c * V, n = p.H - ch;
   const Tokens<LT> k = tokens_of<LT, PACKED>(p, tile * kScanTile + slot * LT);
   // after token i, h = A[i] h_in + B[i], of the state that enters the slot
   float A[LT][V], B[LT][V];
@@ -463,7 +522,12 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 4) void scan_fwd_kernel(ScanArgs
   if (n <= 0) return;
   float h[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) h[v] = sm.enter(slot, c * V + v, LOOK ? lb.enter[c * V + v] : 0.f);
+  for (int v = 0; v < V; ++v) {
+    const int at = Scan<T>::place(c, v);
+    float enter = 0.f;
+    if constexpr (LOOK) enter = lb.enter[at];
+    h[v] = sm.enter(slot, at, enter);
+  }
   // the backward starts its tiles from these
   if (p.states != nullptr && slot == 0) {
     Vec<float, V> q;
@@ -497,13 +561,15 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 4) void scan_fwd_kernel(ScanArgs
 // sequences. The states are run again from what entered the tile.
 template <class T, class G, int FORM, bool PACKED, bool LOOK>
 __global__ __launch_bounds__(Scan<T>::kThreads, 3) void scan_bwd_kernel(ScanArgs p) {
-  constexpr int V = Scan<T>::V, CB = Scan<T>::CB, LT = kScanTokens, NT = Scan<T>::kThreads;
-  __shared__ SlotMaps<CB, NT> sf, sr;
-  __shared__ LookBack<LOOK ? CB : NT, NT> lb;
+  constexpr int V = Scan<T>::V, CB = Scan<T>::CB, LT = kScanTokens;
+  __shared__ SlotMaps<T> sf, sr;
+  __shared__ typename std::conditional<LOOK, LookBack<T>, NoLookBack>::type lb;
   const int c = threadIdx.x % Scan<T>::kLanes, slot = threadIdx.x / Scan<T>::kLanes;
-  const unsigned id = LOOK ? take_ticket(p) : blockIdx.x;
-  const int l = id / p.cblocks, tile = (int)p.ntiles - 1 - l;
-  const int c0 = id % p.cblocks * CB, ch = c0 + c * V, n = p.H - ch;
+  int l, cblock;
+  take_tile<LOOK>(p, l, cblock);
+  if (cblock >= p.cblocks) return;  // the last range may be short
+  const int tile = (int)p.ntiles - 1 - l;
+  const int c0 = cblock * CB, ch = c0 + c * V, n = p.H - ch;
   const Tokens<LT> k = tokens_of<LT, PACKED>(p, tile * kScanTile + slot * LT);
   Vec<T, V> x[LT], go[LT];
   Vec<G, V> g[LT];
@@ -582,8 +648,11 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 3) void scan_bwd_kernel(ScanArgs
     float h[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      h[v] = sf.enter(slot, c * V + v, q.get(v));
-      e[v] = sr.enter(kScanSlots - 1 - slot, c * V + v, LOOK ? lb.enter[c * V + v] : 0.f);
+      const int at = Scan<T>::place(c, v);
+      h[v] = sf.enter(slot, at, q.get(v));
+      float enter = 0.f;
+      if constexpr (LOOK) enter = lb.enter[at];
+      e[v] = sr.enter(kScanSlots - 1 - slot, at, enter);
     }
 #pragma unroll
     for (int i = 0; i < LT; ++i) {
@@ -643,14 +712,14 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 3) void scan_bwd_kernel(ScanArgs
   }
 }
 
-// Before the scan: no words, the first ticket; for packed tokens their marks (the
+// Before the scan: no words, the first tiles' tickets; for packed tokens their marks (the
 // last sequence that starts at or before a token, by bisection: any boundaries
 // give marks in range, ascending ones the right ones), and dst = src for the
 // empty sequences, which no token writes (all of them without tokens).
 __global__ __launch_bounds__(256) void scan_prep_kernel(ScanPrep p) {
   const long long i0 = (long long)blockIdx.x * 256 + threadIdx.x, step = (long long)gridDim.x * 256;
   for (long long i = i0; i < p.nwords; i += step) p.words[i] = kNoWord;
-  if (i0 == 0 && p.ticket != nullptr) *p.ticket = 0;
+  if (p.tickets != nullptr && i0 < kScanRanges) p.tickets[i0 * kTicketStride] = 0;
   if (p.marks != nullptr)
     for (long long t = i0; t < p.N; t += step) {
       int lo = 0, hi = p.S + 1;  // first index whose boundary lies behind t
@@ -749,10 +818,14 @@ hipError_t with_form(int form, bool packed, F&& f) {
 
 }  // namespace
 
-void scan_tiles(int x_type, long long N, int H, long long* ntiles, int* cblocks) {
+void scan_tiles(int x_type, long long N, int H, ScanArgs* a) {
   const int cb = x_type == LTC_F32 ? Scan<float>::CB : Scan<__bf16>::CB;
-  *ntiles = (N + kScanTile - 1) / kScanTile;
-  *cblocks = (H + cb - 1) / cb;
+  a->ntiles = (N + kScanTile - 1) / kScanTile;
+  a->cblocks = (H + cb - 1) / cb;
+  a->per = (a->cblocks + kScanRanges - 1) / kScanRanges;
+  // 512 bytes of a row side by side where there are as many
+  if (a->per < 4) a->per = a->cblocks < 4 ? a->cblocks : 4;
+  a->ranges = (a->cblocks + a->per - 1) / a->per;
 }
 
 // Whether states pass from tile to tile.
@@ -771,7 +844,7 @@ hipError_t launch_scan_prep(const ScanPrep& p, hipStream_t s) {
 }
 
 hipError_t launch_scan(const ScanTypes& ty, const ScanArgs& a, bool bwd, hipStream_t s) {
-  const dim3 grid((unsigned)(a.ntiles * a.cblocks));
+  const dim3 grid((unsigned)(a.ntiles * a.per * a.ranges));
   const bool look = scan_looks(a.N, a.T, a.marks != nullptr);
   return with_types(ty.x, ty.g, [&](auto t, auto g) {
     return with_form(ty.form, a.marks != nullptr, [&](auto form, auto packed) {

@@ -55,11 +55,10 @@ int check_scan(int B, int T, int H, int packed) {
   // sequence numbers share a word with two flags
   if (B > INT_MAX / 4 - 1) return host_fail(LTC_EUNSUPPORTED, "too many sequences");
   const long long N = tokens_in_all(B, T, packed);
-  long long ntiles;
-  int cblocks;
-  ltc::scan_tiles(LTC_F32, N, H, &ntiles, &cblocks);  // the type with the most blocks
+  ltc::ScanArgs t{};
+  ltc::scan_tiles(LTC_F32, N, H, &t);  // the type with the most blocks of channels
   // token numbers are 32-bit, up to a tile behind the last
-  if (N > INT_MAX - 2 * ltc::kScanTile || ntiles > kMaxGroups / cblocks || (long long)B > kMaxGroups * 256 / H)
+  if (N > INT_MAX - 2 * ltc::kScanTile || t.ntiles > kMaxGroups / (t.per * t.ranges) || (long long)B > kMaxGroups * 256 / H)
     return host_fail(LTC_EUNSUPPORTED, "problem too large");
   return LTC_OK;
 }
@@ -80,7 +79,7 @@ ScanSaved carve_saved(Pieces& c, long long N, int H, int packed) {
 struct ScanWs {
   unsigned long long* words;
   long long nwords;
-  unsigned* ticket;
+  unsigned* tickets;
   int* marks;
 };
 ScanWs carve_ws(Pieces& c, long long N, int T, int H, int packed, bool bwd) {
@@ -89,7 +88,7 @@ ScanWs carve_ws(Pieces& c, long long N, int T, int H, int packed, bool bwd) {
   if (N > 0 && ltc::scan_looks(N, T, packed != 0)) {
     w.nwords = (tiles_of(N) + tiles_of(N) / ltc::kScanGroup) * H;
     w.words = c.take<unsigned long long>(w.nwords);
-    w.ticket = c.take<unsigned>(1);
+    w.tickets = c.take<unsigned>(ltc::kScanRanges * ltc::kTicketStride);
   }
   return w;
 }
@@ -244,13 +243,13 @@ int ltc_gated_scan_forward(const void* x, long long sxb, long long sxt, const vo
   a.hf = state_final;
   a.states = sv.states;
   a.words = w.words;
-  a.ticket = w.ticket;
-  ltc::scan_tiles(x_type, N, H, &a.ntiles, &a.cblocks);
+  a.tickets = w.tickets;
+  ltc::scan_tiles(x_type, N, H, &a);
   int* marks = save ? sv.marks : w.marks;
   a.cu = cu_seqlens;
   a.marks = marks;
   const bool ends = B > 0 && (packed || N == 0);
-  const ltc::ScanPrep pr{w.words, w.nwords, w.ticket, cu_seqlens, marks, B, H, N, state,
+  const ltc::ScanPrep pr{w.words, w.nwords, w.tickets, cu_seqlens, marks, B, H, N, state,
                          ends ? state_final : nullptr};
   const hipError_t e = host_timed(ltc::K_SCAN_FWD, [&] {
     hipError_t e = hipSuccess;
@@ -302,13 +301,13 @@ int ltc_gated_scan_backward(const void* x, long long sxb, long long sxt, const v
   a.N = N;
   a.states = sv.states;
   a.words = w.words;
-  a.ticket = w.ticket;
-  ltc::scan_tiles(x_type, N, H, &a.ntiles, &a.cblocks);
+  a.tickets = w.tickets;
+  ltc::scan_tiles(x_type, N, H, &a);
   a.gx = grad_x;
   a.gg = grad_gate;
   a.gs = grad_state;
   const bool ends = B > 0 && grad_state && (packed || N == 0);
-  const ltc::ScanPrep pr{w.words, w.nwords, w.ticket, cu_seqlens, nullptr, B, H, N, grad_state_final,
+  const ltc::ScanPrep pr{w.words, w.nwords, w.tickets, cu_seqlens, nullptr, B, H, N, grad_state_final,
                          ends ? grad_state : nullptr};
   const hipError_t e = host_timed(ltc::K_SCAN_BWD, [&] {
     hipError_t e = hipSuccess;

@@ -21,7 +21,10 @@ constexpr int kScanSlots = 32;
 constexpr int kScanTokens = 4;
 constexpr int kScanTile = kScanSlots * kScanTokens;
 // Tiles whose maps are composed into one.
-constexpr int kScanGroup = 32;
+constexpr int kScanGroup = 16;
+// Ranges of channel blocks, and the words between their counters.
+constexpr int kScanRanges = 8;
+constexpr int kTicketStride = 64;
 
 struct ScanArgs {
   const void* x;
@@ -36,11 +39,12 @@ struct ScanArgs {
   long long N;       // tokens in all
   long long ntiles;
   int cblocks;       // blocks of channels
+  int per, ranges;   // blocks of a range, ranges (take_tile)
   void* out;         // forward (N,H)
   float* hf;         // forward (B,H)
   float* states;     // what enters each tile (ntiles,H); forward: may be null
   unsigned long long* words;  // maps of tiles (ntiles,H), then of groups of tiles
-  unsigned* ticket;
+  unsigned* tickets;  // one for each range of channel blocks, every kTicketStride words
   void* gx;          // backward (N,H), or null where not wanted
   void* gg;          // backward (N,H), or null
   float* gs;         // backward (B,H), or null
@@ -53,7 +57,7 @@ struct ScanTypes {
 struct ScanPrep {
   unsigned long long* words;
   long long nwords;
-  unsigned* ticket;
+  unsigned* tickets;
   const int* cu;
   int* marks;
   int S, H;
@@ -62,7 +66,8 @@ struct ScanPrep {
   float* dst;
 };
 
-void scan_tiles(int x_type, long long N, int H, long long* ntiles, int* cblocks);
+// The tiles of a call: fills in ntiles, cblocks, per and ranges.
+void scan_tiles(int x_type, long long N, int H, ScanArgs* a);
 bool scan_looks(long long N, int T, bool packed);
 hipError_t launch_scan_prep(const ScanPrep& p, hipStream_t s);
 hipError_t launch_scan(const ScanTypes& ty, const ScanArgs& a, bool bwd, hipStream_t s);
