@@ -398,7 +398,8 @@ int ltc_token_logprobs_backward(const void* logits, long long sl, const void* id
  *                1 <= K <= LTC_TEACHER_MAX
  *   loss         (N) fp32; 0 for a row without entries, or whose entries' logits are
  *                all -inf
- * The backward gives dL/dlogits from grad_loss (N), stride sgl; the teacher gets none.
+ * The backward gives dL/dlogits from grad_loss (N), stride sgl, and the forward's
+ * stats, (N,4) fp32 or NULL there; the teacher gets none.
  */
 #define LTC_TEACHER_MAX 1024
 long long ltc_top_distill_workspace_bytes(long long N, int V, int logits_type);

@@ -18,6 +18,7 @@
 
 #include "../../include/ltc_capi.h"
 #include "ltc_seq_internal.h"
+#include "ltc_vec.h"
 
 namespace ltc {
 namespace {
@@ -27,74 +28,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Marks of packed tokens: -1 behind the last sequence (and before the first),
 // else 4 * sequence + 1 for its first token + 2 for its last.
 constexpr int kMarkNone = -1, kMarkStart = 1, kMarkEnd = 2;
-
-// V values of a type, kept packed in words of 32 bits.
-template <class T, int V>
-struct Vec {
-  static constexpr int kWords = V * (int)sizeof(T) / 4;
-  static_assert(kWords * 4 == V * (int)sizeof(T), "whole words");
-  unsigned w[kWords];
-
-  __device__ __forceinline__ float get(int v) const {
-    if constexpr (sizeof(T) == 4) {
-      return __uint_as_float(w[v]);
-    } else if constexpr (std::is_same<T, __bf16>::value) {
-      return __uint_as_float(v & 1 ? w[v / 2] & 0xffff0000u : w[v / 2] << 16);
-    } else {
-      const unsigned short h = (unsigned short)(v & 1 ? w[v / 2] >> 16 : w[v / 2]);
-      return (float)__builtin_bit_cast(_Float16, h);
-    }
-  }
-  // Rounded to nearest, ties to even; the packed conversions take two.
-  __device__ __forceinline__ void put(const float (&f)[V]) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) w[v] = __float_as_uint(f[v]);
-    } else {
-      typedef float F2 __attribute__((ext_vector_type(2)));
-      typedef T T2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-      for (int v = 0; v < V; v += 2) {
-        const F2 q = {f[v], f[v + 1]};
-        w[v / 2] = __builtin_bit_cast(unsigned, __builtin_convertvector(q, T2));
-      }
-    }
-  }
-};
-
-// n (< V: the row's last channels) of V values at p, which has T's alignment
-// only: gfx950 takes wide global loads and stores at any address.
-template <class T, int V>
-__device__ __forceinline__ Vec<T, V> load_vec(const T* p, int n) {
-  Vec<T, V> r;
-  if (n >= V) {
-    __builtin_memcpy(r.w, p, sizeof(r.w));
-  } else {
-#pragma unroll
-    for (int i = 0; i < Vec<T, V>::kWords; ++i) r.w[i] = 0;
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (v < n) {
-        if constexpr (sizeof(T) == 4) r.w[v] = reinterpret_cast<const unsigned*>(p)[v];
-        else r.w[v / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(p)[v] << (v & 1) * 16;
-      }
-  }
-  return r;
-}
-
-template <class T, int V>
-__device__ __forceinline__ void store_vec(T* p, const Vec<T, V>& r, int n) {
-  if (n >= V) {
-    __builtin_memcpy(p, r.w, sizeof(r.w));
-  } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (v < n) {
-        if constexpr (sizeof(T) == 4) reinterpret_cast<unsigned*>(p)[v] = r.w[v];
-        else reinterpret_cast<unsigned short*>(p)[v] = (unsigned short)(r.w[v / 2] >> (v & 1) * 16);
-      }
-  }
-}
 
 // a and 1 - a (decay: 1), each to its own relative precision: with e = exp(-g),
 // a = 1 / (1 + e) and 1 - a = e a. e is kept below 2^126, where a is 2^-126 and
@@ -747,19 +680,35 @@ constexpr int kStepThreads = 256, kStepChannels = 4;
 
 // One token of each row, its state updated in place. A row whose slot an
 // earlier row names too is left to that row, which takes the rows of its slot
-// one after the other, as tokens of one stream.
+// one after the other, as tokens of one stream. Bound by latency: the loads are
+// under way before the workgroup has looked through the slots for its own.
 template <class T, class G, int FORM>
 __global__ __launch_bounds__(kStepThreads) void scan_step_kernel(StepArgs p) {
   constexpr int V = kStepChannels;
   const int row = blockIdx.y;
   const int ch = (blockIdx.x * kStepThreads + threadIdx.x) * V;
   const int n = p.H - ch;
-  int slot = row;
+  const int slot = p.slots != nullptr ? p.slots[row] : row;
+  const bool live = slot >= 0 && slot < p.P;
+  Vec<T, V> x{};
+  Vec<G, V> g{};
+  Vec<float, V> s{};
+  if (n > 0 && live) {
+    x = load_vec<T, V>(static_cast<const T*>(p.x) + row * p.sxb + ch, n);
+    g = load_vec<G, V>(static_cast<const G*>(p.g) + row * p.sgb + ch, n);
+    s = load_vec<float, V>(p.state + slot * p.ssp + ch, n);
+  }
+  T* out = static_cast<T*>(p.out) + ch;
+  int more = 0;  // whether later rows name the slot
   if (p.slots != nullptr) {
-    slot = p.slots[row];
     int earlier = 0;
-    for (int r = threadIdx.x; r < row; r += kStepThreads) earlier |= p.slots[r] == slot;
-    const bool live = slot >= 0 && slot < p.P;
+    for (int r = threadIdx.x; r < p.B; r += kStepThreads) {
+      const bool same = p.slots[r] == slot;
+      earlier |= same && r < row;
+      more |= same && r > row;
+    }
+    earlier = __syncthreads_or(earlier);
+    more = __syncthreads_or(more);
     if (!live) {
       // padding gives zeros, a slot that is not there NaN
       float f[V];
@@ -767,35 +716,37 @@ __global__ __launch_bounds__(kStepThreads) void scan_step_kernel(StepArgs p) {
       for (int v = 0; v < V; ++v) f[v] = slot < 0 ? 0.f : __builtin_nanf("");
       Vec<T, V> o;
       o.put(f);
-      if (n > 0) store_vec<T, V>(static_cast<T*>(p.out) + (long long)row * p.H + ch, o, n);
+      if (n > 0) store_vec<T, V>(out + (long long)row * p.H, o, n);
+      return;
     }
-    if (__syncthreads_or(earlier) || !live) return;
+    if (earlier) return;
   }
   if (n <= 0) return;
-  float* sp = p.state + slot * p.ssp + ch;
-  Vec<float, V> h = load_vec<float, V>(sp, n);
-  for (int r = row; r < p.B; ++r) {
-    if (r > row && (p.slots == nullptr || p.slots[r] != slot)) {
-      if (p.slots == nullptr) break;
-      continue;
-    }
-    const Vec<T, V> x = load_vec<T, V>(static_cast<const T*>(p.x) + r * p.sxb + ch, n);
-    const Vec<G, V> g = load_vec<G, V>(static_cast<const G*>(p.g) + r * p.sgb + ch, n);
-    float f[V];
+  float h[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) h[v] = s.get(v);
+  auto step = [&](int r) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       float a, na;
       gate_of<FORM>(g.get(v), a, na);
-      f[v] = fmaf(a, h.get(v), na * x.get(v));
+      h[v] = fmaf(a, h[v], na * x.get(v));
     }
-    h.put(f);
     Vec<T, V> o;
-    o.put(f);
-    store_vec<T, V>(static_cast<T*>(p.out) + (long long)r * p.H + ch, o, n);
-  }
-  store_vec<float, V>(sp, h, n);
+    o.put(h);
+    store_vec<T, V>(out + (long long)r * p.H, o, n);
+  };
+  step(row);
+  if (more)
+    for (int r = row + 1; r < p.B; ++r) {
+      if (p.slots[r] != slot) continue;
+      x = load_vec<T, V>(static_cast<const T*>(p.x) + r * p.sxb + ch, n);
+      g = load_vec<G, V>(static_cast<const G*>(p.g) + r * p.sgb + ch, n);
+      step(r);
+    }
+  s.put(h);
+  store_vec<float, V>(p.state + slot * p.ssp + ch, s, n);
 }
-
 
 // Calls f with the element types of x and the gate.
 template <class F>

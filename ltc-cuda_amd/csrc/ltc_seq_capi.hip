@@ -134,7 +134,7 @@ int check_temperature(float t) {
 }
 
 ltc::TokArgs tok_args(const void* x, long long sx, const void* ids, int id64, int type, long long N, int V,
-                      float temperature) {
+                      int top, float temperature) {
   ltc::TokArgs a{};
   a.x = x;
   a.sx = sx;
@@ -146,7 +146,8 @@ ltc::TokArgs tok_args(const void* x, long long sx, const void* ids, int id64, in
   a.tau = temperature;
   a.inv_tau = 1.f / temperature;
   a.c = (float)(1.4426950408889634 / (double)temperature);
-  ltc::tok_split(N, V, type_bytes(type), &a.nsplit, &a.seg);
+  a.top = top;
+  ltc::tok_split(N, V, type_bytes(type), top, &a.nsplit, &a.seg);
   return a;
 }
 
@@ -160,7 +161,7 @@ long long parts_bytes(long long N, int V, int top, int type) {
   ltc::TokArgs a{};
   a.N = N;
   a.top = top;
-  ltc::tok_split(N, V, type_bytes(type), &a.nsplit, &a.seg);
+  ltc::tok_split(N, V, type_bytes(type), top, &a.nsplit, &a.seg);
   Pieces c{nullptr};
   carve_parts(c, a);
   return c.off;
@@ -358,8 +359,7 @@ int ltc_token_logprobs_forward(const void* logits, long long sl, const void* ids
   rc = check_workspace(parts_bytes(N, V, top, logits_type), workspace, workspace_bytes);
   if (rc != LTC_OK) return rc;
   if (N == 0) return LTC_OK;
-  ltc::TokArgs a = tok_args(logits, sl, ids, ids64 != 0, logits_type, N, V, temperature);
-  a.top = top;
+  ltc::TokArgs a = tok_args(logits, sl, ids, ids64 != 0, logits_type, N, V, top, temperature);
   a.logp = logp;
   a.ent = entropy;
   a.top_logp = top_logp;
@@ -384,7 +384,7 @@ int ltc_token_logprobs_backward(const void* logits, long long sl, const void* id
   if (N == 0) return LTC_OK;
   if (!logits || !ids || !stats || !grad_logits)
     return host_fail(LTC_EINVAL, "logits/ids/stats/grad_logits pointer is NULL");
-  ltc::TokArgs a = tok_args(logits, sl, ids, ids64 != 0, logits_type, N, V, temperature);
+  ltc::TokArgs a = tok_args(logits, sl, ids, ids64 != 0, logits_type, N, V, 0, temperature);
   a.stats = const_cast<float*>(stats);
   a.gp = grad_logp;
   a.sgp = slp;
@@ -414,7 +414,7 @@ int ltc_top_distill_forward(const void* logits, long long sl, const void* teache
   rc = check_workspace(parts_bytes(N, V, 0, logits_type), workspace, workspace_bytes);
   if (rc != LTC_OK) return rc;
   if (N == 0) return LTC_OK;
-  ltc::TokArgs a = tok_args(logits, sl, teacher_ids, ids64 != 0, logits_type, N, V, temperature);
+  ltc::TokArgs a = tok_args(logits, sl, teacher_ids, ids64 != 0, logits_type, N, V, 0, temperature);
   a.sid = si;
   a.t = teacher_logits;
   a.st = st;
@@ -442,7 +442,7 @@ int ltc_top_distill_backward(const void* logits, long long sl, const void* teach
   if (N == 0) return LTC_OK;
   if (!stats || !grad_loss || !grad_logits)
     return host_fail(LTC_EINVAL, "stats/grad_loss/grad_logits pointer is NULL");
-  ltc::TokArgs a = tok_args(logits, sl, teacher_ids, ids64 != 0, logits_type, N, V, temperature);
+  ltc::TokArgs a = tok_args(logits, sl, teacher_ids, ids64 != 0, logits_type, N, V, 0, temperature);
   a.sid = si;
   a.t = teacher_logits;
   a.st = st;

@@ -104,7 +104,9 @@ struct TokArgs {
   float tau, inv_tau, c;  // temperature, 1 / temperature, log2(e) / temperature
   float* logp;        // (N); the distillation's loss
   float* ent;         // (N) or null
-  float* stats;       // (N,3): row maximum, log of the sum of exp((x - max)/tau), entropy; or null
+  // (N,3): row maximum, log of the sum of exp((x - max)/tau), entropy. Distillation
+  // (N,4): the same two, the teacher's maximum and its log of the sum. Or null.
+  float* stats;
   float* top_logp;    // (N,top)
   long long* top_ids; // (N,top)
   // workspace of rows split over workgroups
@@ -121,7 +123,7 @@ struct TokArgs {
 };
 
 // Logits per workgroup and workgroups per row.
-void tok_split(long long N, int V, int elem_bytes, int* nsplit, int* seg);
+void tok_split(long long N, int V, int elem_bytes, int top, int* nsplit, int* seg);
 hipError_t launch_logprobs_fwd(int x_type, const TokArgs& a, hipStream_t s);
 hipError_t launch_logprobs_bwd(int x_type, const TokArgs& a, hipStream_t s);
 hipError_t launch_distill_fwd(int x_type, const TokArgs& a, hipStream_t s);

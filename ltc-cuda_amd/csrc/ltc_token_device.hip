@@ -11,8 +11,11 @@
 // before the scaling, so large logits lose nothing to it.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "../../include/ltc_capi.h"
 #include "ltc_seq_internal.h"
+#include "ltc_vec.h"
 
 namespace ltc {
 namespace {
@@ -24,7 +27,9 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -3.402823466e38f;
 constexpr int kWaves = kTokThreads / 64;
 
-// Running statistics in powers of two: s0 = sum 2^z, s1 = sum 2^z z, z = (x - m) c.
+// Running statistics in powers of two: s0 = sum 2^z, s1 = sum 2^z z, z = (x - m) c,
+// c = log2(e) / tau. The difference is taken first: a row of the type's lowest value
+// alone (a mask that leaves nothing) is then uniform, as it is by the definition.
 struct Stat {
   float m, s0, s1;
 };
@@ -70,45 +75,38 @@ __device__ __forceinline__ unsigned long long top_key(float x, int j) {
 __device__ __forceinline__ int key_index(unsigned long long k) { return (int)(0xffffffffu - (unsigned)k); }
 __device__ __forceinline__ float key_value(unsigned long long k) { return from_ordered((unsigned)(k >> 32)); }
 
-__device__ __forceinline__ unsigned long long shfl64(unsigned long long v, int src) {
-  const unsigned lo = __shfl((unsigned)v, src), hi = __shfl((unsigned)(v >> 32), src);
+__device__ __forceinline__ unsigned long long lane64(unsigned long long v, int src) {
+  const unsigned lo = __builtin_amdgcn_readlane((unsigned)v, src);
+  const unsigned hi = __builtin_amdgcn_readlane((unsigned)(v >> 32), src);
   return (unsigned long long)hi << 32 | lo;
 }
+// The lane before's value; 0 in the first.
+__device__ __forceinline__ unsigned from_left(unsigned v) {
+  return __builtin_amdgcn_update_dpp(0u, v, 0x138 /* wave_shr:1 */, 0xf, 0xf, false);
+}
 
-// The best keys a wave has seen, one per lane, descending.
+// The best keys a wave has seen, one per lane, descending: whatever the logits are,
+// it holds them.
 struct TopList {
-  unsigned long long key = 0;  // this lane's
-  float thr = -__builtin_inff();  // value of the last that counts; -inf: none yet
+  unsigned long long key;   // this lane's; 0: none
+  unsigned long long last;  // the last that counts
+  float thr;                // its value; -inf: none yet
 
+  __device__ __forceinline__ void clear() {
+    key = last = 0;
+    thr = -__builtin_inff();
+  }
   __device__ __forceinline__ void insert(unsigned long long k) {
     const int pos = __popcll(__ballot(key > k));
     const int lane = threadIdx.x & 63;
-    const unsigned lo = __shfl_up((unsigned)key, 1), hi = __shfl_up((unsigned)(key >> 32), 1);
-    const unsigned long long up = (unsigned long long)hi << 32 | lo;
+    const unsigned long long up =
+        (unsigned long long)from_left((unsigned)(key >> 32)) << 32 | from_left((unsigned)key);
     key = lane < pos ? key : (lane == pos ? k : up);
   }
-  // Descending order of the lanes' keys (bitonic).
-  __device__ __forceinline__ void sort() {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int k = 2; k <= 64; k <<= 1)
-#pragma unroll
-      for (int j = k >> 1; j > 0; j >>= 1) {
-        const unsigned long long o = shfl64(key, lane ^ j);
-        const bool up = (lane & k) != 0, low = (lane & j) == 0;
-        const bool take = (low != up) ? o > key : o < key;
-        key = take ? o : key;
-      }
-  }
   __device__ __forceinline__ void set_threshold(int top) {
-    const unsigned k = __shfl((unsigned)(key >> 32), top - 1);
-    thr = k == 0 ? -__builtin_inff() : from_ordered(k);
+    last = lane64(key, top - 1);
+    thr = last == 0 ? -__builtin_inff() : key_value(last);
   }
-};
-
-template <class T, int V>
-struct TokVec {
-  T v[V];
 };
 
 // Best `top` of n keys in LDS (any order, 0: none), written in order by rank.
@@ -118,6 +116,7 @@ __device__ __forceinline__ void write_top(const unsigned long long* keys, int n,
     const unsigned long long k = keys[i];
     if (k == 0) continue;
     int rank = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) rank += keys[j] > k;
     if (rank < top) best[rank] = k;
   }
@@ -127,21 +126,36 @@ __device__ __forceinline__ long long id_at(const void* ids, int id64, long long 
   return id64 ? static_cast<const long long*>(ids)[i] : static_cast<const int*>(ids)[i];
 }
 
-// Per thread loops over a segment [j0, j1) of a row: the part before the first
-// 16-byte boundary and the rest by single logits, in between 16 bytes a thread.
-// f(value, index) sees the single ones, fv(vector, first index) the others.
-template <class T, class F1, class FV>
+// A workgroup's walk over a segment [j0, j1) of a row: the part before the first
+// 16-byte boundary and the rest by single logits, in between 16 bytes a thread,
+// UNROLL loads of each thread under way at once. f(value, index, there) sees the
+// single ones, fv(vector, first index, there) the others; every thread of the
+// workgroup comes by the same number of times, so they may use the wave.
+template <int UNROLL, class T, class F1, class FV>
 __device__ __forceinline__ void each_logit(const T* row, int j0, int j1, F1&& f, FV&& fv) {
   constexpr int V = 16 / (int)sizeof(T);
   const int off = (int)(((16 - ((uintptr_t)(row + j0) & 15)) & 15) / sizeof(T));
   const int a = j0 + off < j1 ? j0 + off : j1;
   const int nv = (j1 - a) / V, b = a + nv * V;
-  // the loop's trip count is the same for every thread: f and fv may use the wave
-  for (int i = 0; i < nv; i += kTokThreads) {
+  const T* base = row + a;
+  auto load = [&](int q) {
+    Vec<T, V> r;
+    __builtin_memcpy(r.w, __builtin_assume_aligned(base + (long long)q * V, 16), 16);
+    return r;
+  };
+  int i = 0;
+  for (; i + UNROLL * kTokThreads <= nv; i += UNROLL * kTokThreads) {
+    Vec<T, V> x[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) x[u] = load(i + u * kTokThreads + threadIdx.x);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) fv(x[u], a + (i + u * kTokThreads + (int)threadIdx.x) * V, true);
+  }
+  for (; i < nv; i += kTokThreads) {
     const int q = i + threadIdx.x;
     const bool in = q < nv;
-    TokVec<T, V> x{};
-    if (in) x = *reinterpret_cast<const TokVec<T, V>*>(__builtin_assume_aligned(row + a + (long long)q * V, 16));
+    Vec<T, V> x{};
+    if (in) x = load(q);
     fv(x, a + q * V, in);
   }
   const int head = a - j0, tail = j1 - b;  // below V each
@@ -152,6 +166,170 @@ __device__ __forceinline__ void each_logit(const T* row, int j0, int j1, F1&& f,
     f(in ? (float)row[j] : 0.f, j, in);
   }
 }
+
+// The best of a segment, collected on the walk that forms its statistics. Every
+// thread's largest logit so far is at hand (its running maximum), and the best of a
+// workgroup's are bounded from below by
+//   the least over the waves of each wave's (top / 4)-th largest lane maximum, and
+//   any wave's top-th largest lane maximum,
+// since as many logits reach them. What does not reach the bound is out; what does
+// goes to a list, of which the best are taken by rank at the end. The bound is
+// formed again after 1, 2, 4, ... vectors of a thread; 100 to 200 entries come
+// together. If more than kCollect come together
+// (ties; rising logits; masks that leave little else), a second walk keeps ordered
+// lists instead, which hold whatever the logits are.
+constexpr int kCollect = 512;
+struct TopShared {
+  unsigned long long keys[kCollect], kept[kCollect], best[kTopMax];
+  float bound[kWaves], own[kWaves];
+  int n, nkept;
+};
+struct NoTop {};
+
+// The largest of the wave's values (as ordered() numbers them), its lane's set to 0.
+__device__ __forceinline__ unsigned take_max(unsigned& v) {
+  unsigned m = v;
+  // over rows of 16 lanes, then across them: the last lane has seen all
+#define LTC_DPP_MAX(ctrl)                                                                   \
+  {                                                                                         \
+    const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, ctrl, 0xf, 0xf, false); \
+    m = m > o ? m : o;                                                                      \
+  }
+  LTC_DPP_MAX(0x111)  // row_shr:1
+  LTC_DPP_MAX(0x112)
+  LTC_DPP_MAX(0x114)
+  LTC_DPP_MAX(0x118)
+  LTC_DPP_MAX(0x142)  // row_bcast:15
+  LTC_DPP_MAX(0x143)  // row_bcast:31
+#undef LTC_DPP_MAX
+  m = (unsigned)__builtin_amdgcn_readlane((int)m, 63);
+  const unsigned long long at = __ballot(v == m);
+  if ((threadIdx.x & 63) == (unsigned)(__ffsll((long long)at) - 1)) v = 0;
+  return m;
+}
+
+struct Collect {
+  TopShared& sh;
+  int top;
+  bool full;  // every thread of the workgroup has a vector, more than one
+  float bound = -__builtin_inff();
+  int vectors = 0;                              // of each thread
+  int next = 1;                                 // when the bound is formed again
+
+  __device__ __forceinline__ Collect(TopShared& s, int t, bool f) : sh(s), top(t), full(f) {
+    if (threadIdx.x == 0) sh.n = sh.nkept = 0;
+    if ((int)threadIdx.x < t) sh.best[threadIdx.x] = 0;
+    if (threadIdx.x < kWaves) sh.bound[threadIdx.x] = sh.own[threadIdx.x] = -__builtin_inff();
+    __syncthreads();
+  }
+  // The waves' bounds as they are now. They only rise: one read late is lower, and
+  // holds as well.
+  __device__ __forceinline__ void reread() {
+    asm volatile("" ::: "memory");
+    float low = sh.bound[0], k = sh.own[0];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) {
+      low = fminf(low, sh.bound[i]);
+      k = fmaxf(k, sh.own[i]);
+    }
+    bound = fmaxf(bound, fmaxf(low, k));
+  }
+  // largest: this thread's largest logit so far, or kLowest. All waves come by
+  // together the first time and at the end.
+  __device__ __forceinline__ void raise(float largest, bool end) {
+    const int quarter = (top + kWaves - 1) / kWaves, wave = threadIdx.x >> 6;
+    // a wave without logits would hold the least of the waves down for good
+    const bool begin = next == 1;
+    const int n = begin && !full ? top : quarter;
+    next *= 2;
+    // a thread that has seen nothing over the lowest bounds nothing
+    unsigned q = ordered(largest == kLowest ? -__builtin_inff() : largest), m = 0;
+    for (int i = 0; i < n; ++i) {
+      m = take_max(q);
+      if (i == quarter - 1 && (threadIdx.x & 63) == 0) sh.bound[wave] = from_ordered(m);
+    }
+    if (n == top && (threadIdx.x & 63) == 0) sh.own[wave] = from_ordered(m);
+    if (begin || end) __syncthreads();
+    reread();
+  }
+  // Takes in one value a lane (key 0: none).
+  __device__ __forceinline__ void take(unsigned long long k) {
+    const int lane = threadIdx.x & 63;
+    const unsigned long long mask = __ballot(k != 0);
+    int base = 0;
+    if (lane == 0) base = atomicAdd(&sh.n, (int)__popcll(mask));
+    base = __builtin_amdgcn_readfirstlane(base);
+    const int at = base + (int)__popcll(mask & ((1ull << lane) - 1));
+    if (k != 0 && at < kCollect) sh.keys[at] = k;
+  }
+  template <class T, int V>
+  __device__ __forceinline__ void offer(const Vec<T, V>& q, float largest, float so_far, int j, bool in) {
+    if (++vectors == next) raise(so_far, false);
+    if (!__any(in && !(largest < bound))) return;
+    reread();
+    if (!__any(in && !(largest < bound))) return;
+    unsigned cand = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) cand |= !(q.get(v) < bound) ? 1u << v : 0u;
+    if (!in) cand = 0;
+    while (__any(cand != 0)) {
+      const int at = (__ffs((int)cand) - 1) & (V - 1);
+      take(cand != 0 ? top_key(q.get_at(at), j + at) : 0ull);
+      cand &= cand - 1;
+    }
+  }
+  __device__ __forceinline__ void offer(float y, int j, bool in) {
+    const bool reaches = in && !(y < bound);
+    if (__any(reaches)) take(reaches ? top_key(y, j) : 0ull);
+  }
+  // The best, in sh.best (0 where there are none) after the next barrier.
+  template <class T>
+  __device__ __forceinline__ void finish(const T* x, int j0, int j1, float largest) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    raise(largest, true);  // with a barrier: all entries are in, too
+    int n = sh.n;
+    if (n <= kCollect) {
+      // most entries came in under a lower bound
+      for (int i = threadIdx.x; i < n; i += kTokThreads) {
+        const unsigned long long k = sh.keys[i];
+        if (!(key_value(k) < bound)) sh.kept[atomicAdd(&sh.nkept, 1)] = k;
+      }
+      __syncthreads();
+      n = sh.nkept;
+    } else {
+      TopList tl;
+      tl.clear();
+      auto add = [&](unsigned long long k) {
+        unsigned long long mask = __ballot(k > tl.last);
+        while (mask != 0) {
+          const int src = __ffsll((long long)mask) - 1;
+          mask &= mask - 1;
+          const unsigned long long q = lane64(k, src);
+          if (q > tl.last) {
+            tl.insert(q);
+            tl.set_threshold(top);
+          }
+        }
+      };
+      each_logit<4>(
+          x, j0, j1, [&](float y, int j, bool in) { add(in ? top_key(y, j) : 0ull); },
+          [&](const Vec<T, V>& q, int j, bool in) {
+            bool any = false;
+#pragma unroll
+            for (int v = 0; v < V; ++v) any = any || !(q.get(v) < tl.thr);
+            if (!__any(in && any)) return;
+#pragma unroll
+            for (int v = 0; v < V; ++v) add(in ? top_key(q.get(v), j + v) : 0ull);
+          });
+      __syncthreads();
+      if (lane < top) sh.kept[wave * top + lane] = tl.key;
+      n = kWaves * top;
+      __syncthreads();
+    }
+    write_top(sh.kept, n, top, sh.best);
+  }
+};
 
 // What a row's statistics give, by the threads of one workgroup, all of which
 // call it with the same s.
@@ -181,7 +359,7 @@ __device__ void finish_logprobs(const TokArgs& p, long long row, const Stat& s,
   if ((int)threadIdx.x < p.top) {
     const unsigned long long k = best[threadIdx.x];
     p.top_logp[row * p.top + threadIdx.x] = (key_value(k) - s.m) / p.tau - ls;
-    p.top_ids[row * p.top + threadIdx.x] = key_index(k);
+    p.top_ids[row * p.top + threadIdx.x] = k == 0 ? 0 : key_index(k);  // 0: a row of NaN
   }
 }
 
@@ -274,9 +452,11 @@ __device__ void finish_distill(const TokArgs& p, long long row, const Stat& s, f
   if (threadIdx.x == 0) {
     p.logp[row] = t.bad ? __builtin_nanf("") : p.tau * p.tau * sum;
     if (p.stats) {
-      p.stats[row * 3] = s.m;
-      p.stats[row * 3 + 1] = ls;
-      p.stats[row * 3 + 2] = 0.f;
+      p.stats[row * 4] = s.m;
+      p.stats[row * 4 + 1] = ls;
+      // NaN: no loss; -inf: no entries
+      p.stats[row * 4 + 2] = t.bad ? __builtin_nanf("") : t.m;
+      p.stats[row * 4 + 3] = lt;
     }
   }
 }
@@ -289,53 +469,14 @@ __global__ __launch_bounds__(kTokThreads) void tok_fwd_kernel(TokArgs p) {
   constexpr int V = 16 / (int)sizeof(T);
   __shared__ Stat ws[kWaves];
   __shared__ float w[kWaves];
-  __shared__ unsigned long long keys[TOP ? kWaves * kTopMax : 1], best[TOP ? kTopMax : 1];
+  __shared__ typename std::conditional<TOP, TopShared, NoTop>::type tops;
   const long long row = blockIdx.x / p.nsplit;
   const int sp = blockIdx.x % p.nsplit;
   const int j0 = sp * p.seg, j1 = j0 + p.seg < p.V ? j0 + p.seg : p.V;
   const T* x = static_cast<const T*>(p.x) + row * p.sx;
   const float c = p.c;
   Stat s = no_stat();
-  TopList tl;
-  bool first = true;
-
-  auto offer = [&](const float(&y)[V], int j, bool in, int nv) {
-    // at most one bit per value of this lane
-    unsigned cand = 0;
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (v < nv && in && !(y[v] < tl.thr)) cand |= 1u << v;
-    if (!__any(cand != 0)) return;
-    if (first) {
-      // the lanes' largest values start the list: almost nothing else passes it
-      unsigned long long k = 0;
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (cand >> v & 1) {
-          const unsigned long long q = top_key(y[v], j + v);
-          if (q > k) k = q;
-        }
-      if (k != 0) cand &= ~(1u << (key_index(k) - j));
-      tl.key = k;
-      tl.sort();
-      tl.set_threshold(p.top);
-      first = false;
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const unsigned long long k = (cand >> v & 1) && !(y[v] < tl.thr) ? top_key(y[v], j + v) : 0;
-      unsigned long long mask = __ballot(k != 0);
-      while (mask != 0) {
-        const int src = __ffsll((long long)mask) - 1;
-        mask &= mask - 1;
-        const unsigned long long q = shfl64(k, src);
-        if (q > shfl64(tl.key, p.top - 1)) {
-          tl.insert(q);
-          tl.set_threshold(p.top);
-        }
-      }
-    }
-  };
+  // takes nv values in; the largest of them
   auto add = [&](const float(&y)[V], int nv) {
     float mx = y[0];
 #pragma unroll
@@ -350,21 +491,32 @@ __global__ __launch_bounds__(kTokThreads) void tok_fwd_kernel(TokArgs p) {
         s.s0 += e;
         if constexpr (ENT) s.s1 = fmaf(e, finite_z(z), s.s1);
       }
+    return mx;
   };
-  each_logit(
-      x, j0, j1,
-      [&](float v, int j, bool in) {
-        float y[V] = {v};
-        if (in) add(y, 1);
-        if constexpr (TOP) offer(y, j, in, 1);
-      },
-      [&](const TokVec<T, V>& q, int j, bool in) {
-        float y[V];
+  auto walk = [&](auto&& one, auto&& many) {
+    each_logit<4>(
+        x, j0, j1,
+        [&](float v, int j, bool in) {
+          const float y[V] = {v};
+          if (in) add(y, 1);
+          one(v, j, in);
+        },
+        [&](const Vec<T, V>& q, int j, bool in) {
+          float y[V], mx = 0.f;
 #pragma unroll
-        for (int v = 0; v < V; ++v) y[v] = (float)q.v[v];
-        if (in) add(y, V);
-        if constexpr (TOP) offer(y, j, in, V);
-      });
+          for (int v = 0; v < V; ++v) y[v] = q.get(v);
+          if (in) mx = add(y, V);
+          many(q, mx, j, in);
+        });
+  };
+  if constexpr (TOP) {
+    Collect best(tops, p.top, j1 - j0 >= 2 * V * kTokThreads);
+    walk([&](float v, int j, bool in) { best.offer(v, j, in); },
+         [&](const Vec<T, V>& q, float mx, int j, bool in) { best.offer(q, mx, s.m, j, in); });
+    best.finish(x, j0, j1, s.m);
+  } else {
+    walk([](float, int, bool) {}, [](const Vec<T, V>&, float, int, bool) {});
+  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     Stat b;
@@ -373,20 +525,13 @@ __global__ __launch_bounds__(kTokThreads) void tok_fwd_kernel(TokArgs p) {
     b.s1 = __shfl_xor(s.s1, o);
     s = merge<ENT>(s, b, c);
   }
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  if (lane == 0) ws[wave] = s;
-  if constexpr (TOP)
-    if (lane < p.top) keys[wave * p.top + lane] = tl.key;
+  if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = s;
   __syncthreads();
   s = ws[0];
 #pragma unroll
   for (int i = 1; i < kWaves; ++i) s = merge<ENT>(s, ws[i], c);
-  if constexpr (TOP) {
-    if ((int)threadIdx.x < p.top) best[threadIdx.x] = 0;
-    __syncthreads();
-    write_top(keys, kWaves * p.top, p.top, best);
-    __syncthreads();
-  }
+  const unsigned long long* best = nullptr;
+  if constexpr (TOP) best = tops.best;
   if (p.nsplit == 1) {
     if constexpr (OP == kLogprobs) finish_logprobs<T>(p, row, s, best);
     else finish_distill<T>(p, row, s, w);
@@ -403,11 +548,12 @@ __global__ __launch_bounds__(kTokThreads) void tok_fwd_kernel(TokArgs p) {
 }
 
 // Rows split over workgroups: joins their parts, in their order.
-constexpr int kSplitMax = 64;
+constexpr int kSplitMax = 64, kJoinKeys = 512;
+static_assert(kJoinKeys >= kTopMax && kCollect >= kWaves * kTopMax, "one list at least");
 template <class T, int OP, bool ENT, bool TOP>
 __global__ __launch_bounds__(kTokThreads) void tok_join_kernel(TokArgs p) {
   __shared__ float w[kWaves];
-  __shared__ unsigned long long keys[TOP ? kSplitMax * kTopMax : 1], best[TOP ? kTopMax : 1];
+  __shared__ unsigned long long keys[TOP ? kJoinKeys : 1], best[TOP ? kTopMax : 1];
   const long long row = blockIdx.x;
   const float c = p.c;
   Stat s = no_stat();
@@ -436,7 +582,6 @@ __global__ __launch_bounds__(kTokThreads) void tok_join_kernel(TokArgs p) {
 template <class T, int OP>
 __global__ __launch_bounds__(kTokThreads) void tok_bwd_kernel(TokArgs p) {
   constexpr int V = 16 / (int)sizeof(T);
-  __shared__ float w[kWaves];
   __shared__ float pk[OP == kDistill ? kTeacherMax : 1];
   __shared__ int ik[OP == kDistill ? kTeacherMax : 1];
   const long long row = blockIdx.x / p.nsplit;
@@ -445,7 +590,8 @@ __global__ __launch_bounds__(kTokThreads) void tok_bwd_kernel(TokArgs p) {
   const T* x = static_cast<const T*>(p.x) + row * p.sx;
   T* gx = static_cast<T*>(p.gx) + row * p.V;
   const float c = p.c;
-  const float m = p.stats[row * 3], ls = p.stats[row * 3 + 1], H = p.stats[row * 3 + 2];
+  const float* st = p.stats + row * (OP == kDistill ? 4 : 3);
+  const float m = st[0], ls = st[1];
   // dL/dx_j = p_j (k0 + k1 log2 p_j) + what the named ones add
   float k0, k1 = 0.f, named = 0.f;
   long long id = -1;
@@ -455,52 +601,55 @@ __global__ __launch_bounds__(kTokThreads) void tok_bwd_kernel(TokArgs p) {
     if (id < 0) gl = ge = 0.f;
     if (id >= p.V) gl = __builtin_nanf("");
     named = gl * p.inv_tau;
-    k0 = gl == 0.f && ge == 0.f ? 0.f : -(gl + ge * H) * p.inv_tau;
+    k0 = gl == 0.f && ge == 0.f ? 0.f : -(gl + ge * st[2]) * p.inv_tau;
     k1 = -ge * p.inv_tau * kLn2;
   } else {
-    const Teacher t = teacher_of(p, row, w);
-    const float g = t.bad ? __builtin_nanf("") : (t.some ? p.tau * p.gp[row * p.sgp] : 0.f);
-    const float inv = t.some ? 1.f / t.s : 0.f;
-    for (int k = threadIdx.x; k < p.K; k += kTokThreads) {
-      const long long q = id_at(p.ids, p.id64, row * p.sid + k);
-      const bool there = q >= 0 && q < p.V && t.some;
-      ik[k] = there ? (int)q : -1;
-      pk[k] = there ? __builtin_amdgcn_exp2f((teacher_at(p, row, k) - t.m) * c) * inv : 0.f;
-    }
+    const float tm = st[2];
+    const float g = tm == -__builtin_inff() ? 0.f : tm == tm ? p.tau * p.gp[row * p.sgp] : tm;
     named = -g;
     k0 = g;
   }
+  if (k0 == 0.f && k1 == 0.f) {
+    // a row without anything to add is zero whatever its logits are
+    for (int j = j0 + threadIdx.x; j < j1; j += kTokThreads) gx[j] = (T)0.f;
+    return;
+  }
   const float l2 = ls * kLog2e;
-  // A row without anything to add is zero whatever its logits are.
-  const bool none = k0 == 0.f && k1 == 0.f;
   auto grad = [&](float xj) {
     const float l = fmaf(xj - m, c, -l2);  // log2 p_j
     const float pj = __builtin_amdgcn_exp2f(l);
-    if (none) return 0.f;
     if constexpr (OP == kLogprobs) return pj * fmaf(k1, finite_z(l), k0);
     return pj * k0;
   };
-  const bool same = (((uintptr_t)(x + j0) ^ (uintptr_t)(gx + j0)) & 15) == 0;
-  each_logit(
+  each_logit<4>(
       x, j0, j1, [&](float v, int j, bool in) { if (in) gx[j] = (T)grad(v); },
-      [&](const TokVec<T, V>& q, int j, bool in) {
+      [&](const Vec<T, V>& q, int j, bool in) {
         if (!in) return;
-        TokVec<T, V> o;
+        float o[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) o.v[v] = (T)grad((float)q.v[v]);
-        if (same) *reinterpret_cast<TokVec<T, V>*>(__builtin_assume_aligned(gx + j, 16)) = o;
-        else __builtin_memcpy(gx + j, &o, sizeof(o));
+        for (int v = 0; v < V; ++v) o[v] = grad(q.get(v));
+        Vec<T, V> r;
+        r.put(o);
+        store_vec<T, V>(gx + j, r, V);
       });
-  __syncthreads();
   if constexpr (OP == kLogprobs) {
+    __syncthreads();
     if (threadIdx.x == 0 && id >= j0 && id < j1) gx[id] = (T)(grad((float)x[id]) + named);
   } else {
+    const float tm = st[2], lt = st[3];
+    for (int k = threadIdx.x; k < p.K; k += kTokThreads) {
+      const long long q = id_at(p.ids, p.id64, row * p.sid + k);
+      const bool here = q >= j0 && q < j1;
+      ik[k] = here ? (int)q : -1;
+      pk[k] = here ? __builtin_amdgcn_exp2f(((teacher_at(p, row, k) - tm) / p.tau - lt) * kLog2e) : 0.f;
+    }
+    __syncthreads();
     for (int k = threadIdx.x; k < p.K; k += kTokThreads) {
       const int j = ik[k];
-      if (j < j0 || j >= j1) continue;
+      if (j < 0) continue;
       float sum = 0.f;
       for (int q = 0; q < p.K; ++q) sum += ik[q] == j ? pk[q] : 0.f;
-      gx[j] = (T)(none ? 0.f : fmaf(named, sum, grad((float)x[j])));
+      gx[j] = (T)fmaf(named, sum, grad((float)x[j]));
     }
   }
 }
@@ -523,13 +672,15 @@ hipError_t fwd(const TokArgs& a, hipStream_t s) {
 
 }  // namespace
 
-void tok_split(long long N, int V, int elem_bytes, int* nsplit, int* seg) {
-  // whole rows keep 1024 workgroups busy; fewer are cut, to no less than four
-  // 16-byte loads of every thread
+void tok_split(long long N, int V, int elem_bytes, int top, int* nsplit, int* seg) {
+  // 1024 rows fill the chip; fewer are cut, to no less than four loads of every
+  // thread (one row of 131072 fp32: 9.5 us, with one or two loads 13 us, as the join
+  // then has more to do), and to what the join orders at once.
   const int vec = 16 / elem_bytes, least = 4 * kTokThreads * vec;
   long long n = N < 1 || N >= 1024 ? 1 : (1024 + N - 1) / N;
   if (n > (V + least - 1) / least) n = (V + least - 1) / least;
   if (n > kSplitMax) n = kSplitMax;
+  if (top > 0 && n > kJoinKeys / top) n = kJoinKeys / top;
   if (n < 1) n = 1;
   long long sg = (V + n - 1) / n;
   sg = (sg + vec - 1) / vec * vec;

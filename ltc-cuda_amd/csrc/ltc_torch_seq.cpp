@@ -455,7 +455,7 @@ Tensor top_distill(const Tensor& logits, const Tensor& teacher, const Tensor& id
     const Tensor x = flat(logits, r.N, r.V), t = flat(teacher, r.N, K), id = flat(ids, r.N, K);
     const auto f32 = logits.options().dtype(at::kFloat);
     loss = at::empty(shape, f32);
-    if (needs_grad) stats = at::empty({r.N, 3}, f32);
+    if (needs_grad) stats = at::empty({r.N, 4}, f32);
     const long long bytes = ltc_top_distill_workspace_bytes(r.N, r.V, type_of(logits, "logits"));
     const Workspace ws(bytes, logits);
     check_rc(ltc_top_distill_forward(ptr(x), x.stride(0), ptr(t), t.stride(0), ptr(id), id.stride(0), id64,
