@@ -491,7 +491,9 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 4) void scan_fwd_kernel(ScanArgs
 }
 
 // Backward: the carry from token t + 1 to t is a_{t+1} d_{t+1}, nothing across
-// sequences. The states are run again from what entered the tile.
+// sequences. The states are run again from what entered the tile. Gates are formed
+// three times (for the maps, the states, the gradients): kept, they take 64
+// registers more, which spill.
 template <class T, class G, int FORM, bool PACKED, bool LOOK>
 __global__ __launch_bounds__(Scan<T>::kThreads, 3) void scan_bwd_kernel(ScanArgs p) {
   constexpr int V = Scan<T>::V, CB = Scan<T>::CB, LT = kScanTokens;
@@ -575,7 +577,7 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 3) void scan_bwd_kernel(ScanArgs
   forget(g);
   forget(go);
   if (n <= 0 || k.t0 >= p.N) return;
-  float hp[LT][V], na[LT][V], a[LT][V], e[V];  // state before token i, carry into it
+  float hp[LT][V], e[V];  // state before token i, carry into it
   {
     const Vec<float, V> q = load_vec<float, V>(p.states + (long long)tile * p.H + ch, n);
     float h[V];
@@ -592,13 +594,15 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 3) void scan_bwd_kernel(ScanArgs
       if (k.start >> i & 1) begin_state<V>(p, k, i, ch, n, h);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        gate_of<FORM>(g[i].get(v), a[i][v], na[i][v]);
+        float a, na;
+        gate_of<FORM>(g[i].get(v), a, na);
         const float xv = x[i].get(v);
         hp[i][v] = h[v];
-        h[v] = fmaf(a[i][v], h[v], FORM == LTC_GATE_BLEND ? na[i][v] * xv : xv);
+        h[v] = fmaf(a, h[v], FORM == LTC_GATE_BLEND ? na * xv : xv);
       }
     }
   }
+  forget(g);
   long long at = (long long)k.t0 * p.H + ch + (LT - 1) * (long long)p.H;
 #pragma unroll
   for (int i = LT - 1; i >= 0; --i, at -= p.H) {
@@ -613,11 +617,13 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 3) void scan_bwd_kernel(ScanArgs
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
+      float a, na;
+      gate_of<FORM>(g[i].get(v), a, na);
       const float d = o[v] + e[v];
-      e[v] = ds[v] = a[i][v] * d;
+      e[v] = ds[v] = a * d;
       if constexpr (FORM == LTC_GATE_BLEND) {
-        dx[v] = na[i][v] * d;
-        dg[v] = ds[v] * (na[i][v] * (hp[i][v] - x[i].get(v)));
+        dx[v] = na * d;
+        dg[v] = ds[v] * (na * (hp[i][v] - x[i].get(v)));
       } else {
         dx[v] = d;
         dg[v] = ds[v] * hp[i][v];

@@ -592,6 +592,22 @@ __global__ __launch_bounds__(kTokThreads) void tok_bwd_kernel(TokArgs p) {
   const float c = p.c;
   const float* st = p.stats + row * (OP == kDistill ? 4 : 3);
   const float m = st[0], ls = st[1];
+  // the row's entries are under way while it is walked
+  constexpr int kEntries = OP == kDistill ? kTeacherMax / kTokThreads : 1;
+  long long tid[kEntries];
+  float tl[kEntries];
+  if constexpr (OP == kDistill) {
+#pragma unroll
+    for (int i = 0; i < kEntries; ++i) {
+      const int k = threadIdx.x + i * kTokThreads;
+      tid[i] = -1;
+      tl[i] = 0.f;
+      if (k < p.K) {
+        tid[i] = id_at(p.ids, p.id64, row * p.sid + k);
+        tl[i] = teacher_at(p, row, k);
+      }
+    }
+  }
   // dL/dx_j = p_j (k0 + k1 log2 p_j) + what the named ones add
   float k0, k1 = 0.f, named = 0.f;
   long long id = -1;
@@ -637,19 +653,23 @@ __global__ __launch_bounds__(kTokThreads) void tok_bwd_kernel(TokArgs p) {
     if (threadIdx.x == 0 && id >= j0 && id < j1) gx[id] = (T)(grad((float)x[id]) + named);
   } else {
     const float tm = st[2], lt = st[3];
-    for (int k = threadIdx.x; k < p.K; k += kTokThreads) {
-      const long long q = id_at(p.ids, p.id64, row * p.sid + k);
-      const bool here = q >= j0 && q < j1;
-      ik[k] = here ? (int)q : -1;
-      pk[k] = here ? __builtin_amdgcn_exp2f(((teacher_at(p, row, k) - tm) / p.tau - lt) * kLog2e) : 0.f;
+#pragma unroll
+    for (int i = 0; i < kEntries; ++i) {
+      const int k = threadIdx.x + i * kTokThreads;
+      if (k >= p.K) break;
+      const bool here = tid[i] >= j0 && tid[i] < j1;
+      ik[k] = here ? (int)tid[i] : -1;
+      pk[k] = here ? __builtin_amdgcn_exp2f(((tl[i] - tm) / p.tau - lt) * kLog2e) : 0.f;
     }
     __syncthreads();
     for (int k = threadIdx.x; k < p.K; k += kTokThreads) {
       const int j = ik[k];
       if (j < 0) continue;
+      const float xj = (float)x[j];
       float sum = 0.f;
+#pragma unroll 8
       for (int q = 0; q < p.K; ++q) sum += ik[q] == j ? pk[q] : 0.f;
-      gx[j] = (T)fmaf(named, sum, grad((float)x[j]));
+      gx[j] = (T)fmaf(named, sum, grad(xj));
     }
   }
 }
