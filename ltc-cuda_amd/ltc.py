@@ -20,6 +20,9 @@ one behind the caller's back. CPU tensors, non-fp32 tensors and an explicit
 `module._force_torchscript = True` use the TorchScript loop below, which is
 this module's own CPU implementation of the same equations (the reference
 does the same, ltc.py:293-323).
+
+Beyond the reference: `LinearTimeConstant`, the layer without recurrent synapses, whose
+time axis is parallel, and `TokenReadout`, from states to token scores and losses.
 """
 
 from __future__ import annotations
@@ -340,3 +343,218 @@ class TrueLiquidTimeConstant(nn.Module):
 
 
 TemporalLTC = TrueLiquidTimeConstant
+
+
+def _on_hip(*tensors) -> bool:
+    """Whether the fused operators serve these: HIP tensors go to the library, and a
+    missing library is an error there; CPU tensors take the plain forms below."""
+    return all(t is None or t.is_cuda for t in tensors)
+
+
+def _gated_scan_plain(x, gate, state, cu_seqlens=None):
+    """ltc_cuda.ltc_gated_scan's "blend" form in plain torch, step by step."""
+    if cu_seqlens is None:
+        a, u = torch.sigmoid(gate), torch.sigmoid(-gate) * x
+        h, outs = state, []
+        for t in range(x.shape[1]):
+            h = a[:, t] * h + u[:, t]
+            outs.append(h)
+        return (torch.stack(outs, 1) if outs else torch.zeros_like(x)), h
+    cu = cu_seqlens.tolist()
+    out, finals = [x.new_zeros(cu[0], x.shape[1])], []
+    for s in range(len(cu) - 1):
+        o, h = _gated_scan_plain(x[None, cu[s]:cu[s + 1]], gate[None, cu[s]:cu[s + 1]],
+                                 state[s:s + 1])
+        out.append(o[0])
+        finals.append(h)
+    out.append(x.new_zeros(x.shape[0] - cu[-1], x.shape[1]))
+    return torch.cat(out), (torch.cat(finals) if finals else state)
+
+
+class _ScaleColumns(torch.autograd.Function):
+    """w (D, H) times s (H,). The gradient of s is summed by halves: torch's own
+    reduction over many rows is replayed wrongly in a captured graph."""
+
+    @staticmethod
+    def forward(ctx, w, s):
+        ctx.save_for_backward(w, s)
+        return w * s
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        w, s = ctx.saved_tensors
+        t = g * w
+        t = F.pad(t, (0, 0, 0, (1 << (t.shape[0] - 1).bit_length()) - t.shape[0]))
+        while t.shape[0] > 1:
+            half = t.shape[0] // 2
+            t = t[:half] + t[half:]
+        return g * s, t[0]
+
+
+class LinearTimeConstant(nn.Module):
+    """LTC layer without recurrent synapses: sensory synapses, leak and capacitance only.
+
+    Its implicit-Euler step v' = (cm v + gleak vleak + num) / (cm + gleak + den +
+    epsilon) is a gated linear recurrence, since num and den come from the inputs
+    alone: with G = gleak + den + epsilon, a = cm / (cm + G) = sigmoid(log cm - log G)
+    and v' = a v + (1 - a) (gleak vleak + num) / G. So a whole sequence is one sensory
+    pass over all steps and one ltc_cuda.ltc_gated_scan, parallel in time, where
+    TrueLiquidTimeConstant advances step by step. Same parameter names, constructor
+    arguments and calling convention as that layer, of which it is the case of one
+    unfold and an empty recurrent mask.
+
+    float32, as that layer. forward also takes packed sequences: x_seq (tokens, D)
+    with cu_seqlens (int32, sequences + 1). step() advances streams by one token for serving, their states
+    updated in place, in rows of a pool if slots are given.
+    """
+
+    def __init__(
+        self,
+        input_dim: int,
+        hidden_dim: int = 64,
+        dt: float = 1.0 / 30.0,
+        sensory_sparsity: float = 0.5,
+        input_mapping: str = "affine",
+        epsilon: float = 1e-8,
+    ):
+        super().__init__()
+        self.input_dim = input_dim
+        self.hidden_dim = hidden_dim
+        self.dt = float(dt)
+        self.sensory_sparsity = sensory_sparsity
+        self.input_mapping = input_mapping
+        self.epsilon = epsilon
+        H, D = hidden_dim, input_dim
+        self.sensory_w = nn.Parameter(torch.empty(D, H).uniform_(0.001, 1.0))
+        self.sensory_mu = nn.Parameter(torch.empty(D, H).uniform_(0.3, 0.8))
+        self.sensory_sigma = nn.Parameter(torch.empty(D, H).uniform_(3.0, 8.0))
+        mask, erev = TrueLiquidTimeConstant._create_sensory_wiring(D, H, sensory_sparsity)
+        self.register_buffer("sensory_sparsity_mask", mask)
+        self.sensory_erev = nn.Parameter(erev)
+        self.gleak = nn.Parameter(torch.empty(H).uniform_(0.001, 1.0))
+        self.vleak = nn.Parameter(torch.empty(H).uniform_(-0.2, 0.2))
+        self.cm = nn.Parameter(torch.empty(H).uniform_(0.4, 0.6))
+        w, b = torch.ones(D), torch.zeros(D)
+        if input_mapping in ("affine", "linear"):
+            self.input_w = nn.Parameter(w)
+        else:
+            self.register_buffer("input_w", w)
+        if input_mapping == "affine":
+            self.input_b = nn.Parameter(b)
+        else:
+            self.register_buffer("input_b", b)
+        self.input_norm = nn.LayerNorm(D)
+
+    def _drive(self, x):
+        """Gate and drive of every row: (..., D) -> two (..., H).
+
+        The leak is a synapse from a constant input (sigma 0, so its gate is 1/2), the
+        capacitance scales every conductance, and the input map is part of the
+        LayerNorm's: every parameter's gradient over the rows is then formed by the
+        sensory kernels or the LayerNorm, in the same order each time.
+        """
+        norm = self.input_norm
+        rows = F.layer_norm(x, (self.input_dim,), norm.weight * self.input_w,
+                            norm.bias * self.input_w + self.input_b,
+                            norm.eps).reshape(-1, self.input_dim)
+        gleak = F.softplus(self.gleak)
+        leak = gleak + self.epsilon
+        zero = torch.zeros_like(leak)
+        w_pos = torch.cat([F.softplus(self.sensory_w) * self.sensory_sparsity_mask,
+                           (2.0 * leak)[None]])
+        w_pos = _ScaleColumns.apply(w_pos, self.dt / F.softplus(self.cm))
+        erev = torch.cat([self.sensory_erev, (gleak * self.vleak / leak)[None]])
+        mu = torch.cat([self.sensory_mu, zero[None]])
+        sigma = torch.cat([self.sensory_sigma, zero[None]])
+        rows = F.pad(rows, (0, 1))
+        if _on_hip(rows):
+            num, den = ltc_cuda.ltc_sensory_sums(rows, sigma, mu, w_pos, erev)
+        else:
+            cond = w_pos * torch.sigmoid(sigma * (rows.unsqueeze(-1) - mu))
+            num, den = (cond * erev).sum(1), cond.sum(1)
+        # a = cm / (cm + G) = 1 / (1 + den), the conductances being in units of cm
+        shape = (*x.shape[:-1], self.hidden_dim)
+        return -torch.log(den).view(shape), (num / den).view(shape)
+
+    def forward(self, x_seq, h0=None, cu_seqlens=None):
+        """(B, T, D), or packed (tokens, D) with cu_seqlens -> (outputs, (h, h)).
+
+        h0 is an (h, c) pair as TrueLiquidTimeConstant takes it; only h is used.
+        """
+        state = None if h0 is None else h0[0]
+        gate, drive = self._drive(x_seq)
+        if _on_hip(x_seq):
+            out, h = ltc_cuda.ltc_gated_scan(drive, gate, state, cu_seqlens)
+        else:
+            if state is None:
+                n = x_seq.shape[0] if cu_seqlens is None else cu_seqlens.numel() - 1
+                state = drive.new_zeros(n, self.hidden_dim)
+            out, h = _gated_scan_plain(drive, gate, state, cu_seqlens)
+        return out, (h, h)
+
+    @torch.no_grad()
+    def step(self, x, state, slots=None):
+        """One token of each stream: x (B, D) -> (B, H); `state` (B, H), or a pool
+        whose rows slots (B,) int32 name (negative: padding), is updated in place."""
+        gate, drive = self._drive(x)
+        if _on_hip(x, state):
+            return ltc_cuda.ltc_gated_scan_step(drive, gate, state, slots)
+        out = torch.zeros_like(drive)
+        for b in range(x.shape[0]):
+            s = b if slots is None else int(slots[b])
+            if s >= 0:
+                state[s] = torch.lerp(drive[b], state[s], torch.sigmoid(gate[b]))
+                out[b] = state[s]
+        return out
+
+
+class TokenReadout(nn.Module):
+    """Linear readout of a layer's states to the logits of a vocabulary, and what is
+    asked of them: scores of given tokens, and a teacher's distribution to learn.
+
+    forward(h) -> logits; log_probs(h, ids) -> ltc_cuda.ltc_token_logprobs of them;
+    distill(h, teacher_logits, teacher_ids) -> ltc_cuda.ltc_top_distill's loss of each
+    row. The logits are in the readout's own type (float32, bfloat16 or float16), what
+    is made of them in float32. There is no bias: torch forms its gradient with a
+    reduction that a captured graph replays wrongly. CPU tensors take plain torch.
+    """
+
+    def __init__(self, hidden_dim: int, vocab: int, dtype=None):
+        super().__init__()
+        self.proj = nn.Linear(hidden_dim, vocab, bias=False, dtype=dtype)
+
+    def forward(self, h):
+        return self.proj(h.to(self.proj.weight.dtype))
+
+    def log_probs(self, h, ids, top: int = 0, temperature: float = 1.0):
+        """(log probability, entropy[, top log probabilities, top ids]) of each row."""
+        logits = self(h)
+        if _on_hip(logits):
+            return ltc_cuda.ltc_token_logprobs(logits, ids, top=top, temperature=temperature)
+        lq = torch.log_softmax(logits.float() / temperature, -1)
+        q = lq.exp()
+        ent = -torch.where(q > 0, q * lq, torch.zeros_like(q)).sum(-1)
+        lp = lq.gather(-1, ids.clamp(min=0).long().unsqueeze(-1)).squeeze(-1)
+        zero = torch.zeros_like(ent)
+        res = (torch.where(ids >= 0, lp, zero), torch.where(ids >= 0, ent, zero))
+        if top:
+            order = torch.sort(logits, dim=-1, descending=True, stable=True).indices[..., :top]
+            res += (lq.gather(-1, order).detach(), order)
+        return res
+
+    def distill(self, h, teacher_logits, teacher_ids, temperature: float = 1.0):
+        """Distillation loss of each row against the teacher's best logits."""
+        logits = self(h)
+        if _on_hip(logits):
+            return ltc_cuda.ltc_top_distill(logits, teacher_logits, teacher_ids,
+                                            temperature=temperature)
+        lq = torch.log_softmax(logits.float() / temperature, -1)
+        t = teacher_logits.float() / temperature
+        t = t.masked_fill(teacher_ids < 0, -float("inf"))
+        some = (t > -float("inf")).any(-1, keepdim=True)
+        lp = torch.log_softmax(torch.where(some, t, torch.zeros_like(t)), -1)
+        p = torch.where(some & (t > -float("inf")), lp.exp(), torch.zeros_like(lp))
+        diff = lp - lq.gather(-1, teacher_ids.clamp(min=0).long())
+        return temperature ** 2 * torch.where(p > 0, p * diff, torch.zeros_like(p)).sum(-1)
+

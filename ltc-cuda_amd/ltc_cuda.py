@@ -851,6 +851,28 @@ def ltc_cuda_forward(x_seq, state, w_pos, w_erev, mu, sigma,
         cm_t, gleak_pos, vleak, ode_unfolds, epsilon, needs_grad)
 
 
+class LTCSensoryFunction(torch.autograd.Function):
+    """The sensory sums of every row, [w_num, w_den] (N, H), with their gradients: the
+    per-step entry points ltc_sensory_fwd / ltc_sensory_bwd over all rows at once."""
+
+    @staticmethod
+    def forward(ctx, inputs, sigma, mu, w_pos, erev):
+        ctx.save_for_backward(inputs, sigma, mu, w_pos, erev)
+        return tuple(require_kernels().ltc_sensory_fwd(inputs, sigma, mu, w_pos, erev))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_num, g_den):
+        g = require_kernels().ltc_sensory_bwd(g_num, g_den, *ctx.saved_tensors)
+        return tuple(g)
+
+
+def ltc_sensory_sums(inputs, sigma, mu, w_pos, erev):
+    """Sensory sums of rows (N, D) -> (w_num, w_den) (N, H), with gradients:
+    sum_d w_pos sigmoid(sigma (x - mu)) erev, and the same without erev."""
+    return LTCSensoryFunction.apply(inputs, sigma, mu, w_pos, erev)
+
+
 # ------------------------------------------------ sequence and token operators
 
 # ltc_gated_scan's gates, as include/ltc_capi.h numbers them.
