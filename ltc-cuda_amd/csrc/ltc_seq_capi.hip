@@ -32,8 +32,7 @@ struct Pieces {
 };
 
 int check_workspace(long long need, const void* ws, long long have) {
-  if (need == 0) return LTC_OK;
-  if (ws == nullptr || have < need)
+  if (need > 0 && (ws == nullptr || have < need))
     return host_fail(LTC_EINVAL, "workspace too small: need " + std::to_string(need) + " bytes, got " +
                                      std::to_string(ws ? have : 0));
   if (reinterpret_cast<uintptr_t>(ws) % 256 != 0)

@@ -405,8 +405,8 @@ class LinearTimeConstant(nn.Module):
     unfold and an empty recurrent mask.
 
     float32, as that layer. forward also takes packed sequences: x_seq (tokens, D)
-    with cu_seqlens (int32, sequences + 1). step() advances streams by one token for serving, their states
-    updated in place, in rows of a pool if slots are given.
+    with cu_seqlens (int32, sequences + 1). step() advances streams by one token for
+    serving, their states updated in place, in rows of a pool if slots are given.
     """
 
     def __init__(

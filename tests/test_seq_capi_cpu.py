@@ -50,7 +50,9 @@ def _bwd(lib, x=1, gate=1, cu=None, xt=0, gt=0, form=0, B=2, T=3, H=4, saved=1, 
 
 
 def test_scan_refusals(lib):
-    need = lib.lib.ltc_gated_scan_fwd_workspace_bytes(2, 3, 4, 0)
+    # sequences longer than a tile hand states on through the workspace
+    need = lib.lib.ltc_gated_scan_fwd_workspace_bytes(2, 400, 4, 0)
+    assert need > 0 and lib.lib.ltc_gated_scan_fwd_workspace_bytes(2, 3, 4, 0) == 0
     for call in (_fwd, _bwd):
         for kw, what in (({"H": 0}, "H >= 1"), ({"B": -1}, "B >= 0"), ({"T": -2}, "T >= 0"),
                          ({"xt": 3}, "x_type"), ({"xt": -1}, "x_type"), ({"gt": 1}, "gate_type"),
@@ -59,9 +61,9 @@ def test_scan_refusals(lib):
             assert call(lib, **kw) == 1, (call.__name__, kw)
             assert what in lib.last_error(), (kw, lib.last_error())
         assert call(lib, B=INT_MAX // 8, T=INT_MAX) == 2
-    if need:
-        assert _fwd(lib, wsb=need - 1) == 1 and "too small" in lib.last_error()
-        assert _fwd(lib, ws=None) == 1 and "too small" in lib.last_error()
+    assert _fwd(lib, T=400, wsb=need - 1) == 1 and "too small" in lib.last_error()
+    assert _fwd(lib, T=400, ws=None) == 1 and "too small" in lib.last_error()
+    assert _bwd(lib, T=400, ws=None) == 1 and "too small" in lib.last_error()
     assert _fwd(lib, out=None) == 1 and "out" in lib.last_error()
     assert _fwd(lib, hf=None) == 1 and "state_final" in lib.last_error()
     assert _fwd(lib, save=1) == 1 and "saved" in lib.last_error()
