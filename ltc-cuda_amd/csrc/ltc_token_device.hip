@@ -57,6 +57,20 @@ __device__ __forceinline__ Stat merge(Stat a, Stat b, float c) {
   return a;
 }
 
+// Of all lanes, in every lane.
+template <bool ENT>
+__device__ __forceinline__ Stat merge_wave(Stat s, float c) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    Stat b;
+    b.m = __shfl_xor(s.m, o);
+    b.s0 = __shfl_xor(s.s0, o);
+    b.s1 = __shfl_xor(s.s1, o);
+    s = merge<ENT>(s, b, c);
+  }
+  return s;
+}
+
 // Order of alternatives as one integer: larger logits first (NaN before all),
 // equal ones by the lower index. 0 is no entry.
 __device__ __forceinline__ unsigned ordered(float x) {
@@ -517,14 +531,7 @@ __global__ __launch_bounds__(kTokThreads) void tok_fwd_kernel(TokArgs p) {
   } else {
     walk([](float, int, bool) {}, [](const Vec<T, V>&, float, int, bool) {});
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    Stat b;
-    b.m = __shfl_xor(s.m, o);
-    b.s0 = __shfl_xor(s.s0, o);
-    b.s1 = __shfl_xor(s.s1, o);
-    s = merge<ENT>(s, b, c);
-  }
+  s = merge_wave<ENT>(s, c);
   if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = s;
   __syncthreads();
   s = ws[0];
@@ -547,32 +554,50 @@ __global__ __launch_bounds__(kTokThreads) void tok_fwd_kernel(TokArgs p) {
   }
 }
 
-// Rows split over workgroups: joins their parts, in their order.
+// Rows split over workgroups: joins their parts, a lane of each wave to a part.
 constexpr int kSplitMax = 64, kJoinKeys = 512;
 static_assert(kJoinKeys >= kTopMax && kCollect >= kWaves * kTopMax, "one list at least");
 template <class T, int OP, bool ENT, bool TOP>
 __global__ __launch_bounds__(kTokThreads) void tok_join_kernel(TokArgs p) {
   __shared__ float w[kWaves];
-  __shared__ unsigned long long keys[TOP ? kJoinKeys : 1], best[TOP ? kTopMax : 1];
+  __shared__ unsigned long long keys[TOP ? kJoinKeys : 1], kept[TOP ? kJoinKeys : 1], best[TOP ? kTopMax : 1];
+  __shared__ int nkept;
   const long long row = blockIdx.x;
-  const float c = p.c;
+  const int lane = threadIdx.x & 63;
   Stat s = no_stat();
-  for (int i = 0; i < p.nsplit; ++i) {
-    const float* q = p.part + (row * p.nsplit + i) * 3;
-    Stat b;
-    b.m = q[0];
-    b.s0 = q[1];
-    b.s1 = q[2];
-    s = merge<ENT>(s, b, c);
+  if (lane < p.nsplit) {
+    const float* q = p.part + (row * p.nsplit + lane) * 3;
+    s.m = q[0];
+    s.s0 = q[1];
+    s.s1 = q[2];
   }
   if constexpr (TOP) {
     const int n = p.nsplit * p.top;
     for (int i = threadIdx.x; i < n; i += kTokThreads) keys[i] = p.part_top[row * n + i];
     if ((int)threadIdx.x < p.top) best[threadIdx.x] = 0;
+    if (threadIdx.x == 0) nkept = 0;
     __syncthreads();
-    write_top(keys, n, p.top, best);
+    // The parts' lists are in order. As many keys as are wanted reach the least of
+    // their (top / parts)-th, and the last of any (by rank over all 500 keys of 25
+    // parts this took 19 us).
+    const int share = (p.top + p.nsplit - 1) / p.nsplit;
+    unsigned long long low = ~0ull, bound = 0;
+#pragma unroll 8
+    for (int i = 0; i < p.nsplit; ++i) {
+      const unsigned long long k = keys[i * p.top + share - 1], l = keys[(i + 1) * p.top - 1];
+      low = k < low ? k : low;
+      bound = l > bound ? l : bound;
+    }
+    bound = low > bound ? low : bound;
+    for (int i = threadIdx.x; i < n; i += kTokThreads) {
+      const unsigned long long k = keys[i];
+      if (k >= bound && k != 0) kept[atomicAdd(&nkept, 1)] = k;
+    }
+    __syncthreads();
+    write_top(kept, nkept, p.top, best);
     __syncthreads();
   }
+  s = merge_wave<ENT>(s, p.c);
   if constexpr (OP == kLogprobs) finish_logprobs<T>(p, row, s, best);
   else finish_distill<T>(p, row, s, w);
 }
@@ -693,10 +718,10 @@ hipError_t fwd(const TokArgs& a, hipStream_t s) {
 }  // namespace
 
 void tok_split(long long N, int V, int elem_bytes, int top, int* nsplit, int* seg) {
-  // 1024 rows fill the chip; fewer are cut, to no less than four loads of every
-  // thread (one row of 131072 fp32: 9.5 us, with one or two loads 13 us, as the join
-  // then has more to do), and to what the join orders at once.
-  const int vec = 16 / elem_bytes, least = 4 * kTokThreads * vec;
+  // 1024 rows fill the chip; fewer are cut, to no less than one load of every thread
+  // (8 rows of 32000 bf16: 6.3 us in both launches with one, 6.9 with four; top 20
+  // 14.2 and 15.1), and to what the join orders at once.
+  const int vec = 16 / elem_bytes, least = kTokThreads * vec;
   long long n = N < 1 || N >= 1024 ? 1 : (1024 + N - 1) / N;
   if (n > (V + least - 1) / least) n = (V + least - 1) / least;
   if (n > kSplitMax) n = kSplitMax;
