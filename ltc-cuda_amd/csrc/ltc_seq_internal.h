@@ -23,7 +23,7 @@ constexpr int kScanTile = kScanSlots * kScanTokens;
 // Tiles whose maps are composed into one.
 constexpr int kScanGroup = 16;
 // Ranges of channel blocks, and the words between their counters.
-constexpr int kScanRanges = 8;
+constexpr int kScanRanges = 7;
 constexpr int kTicketStride = 64;
 
 struct ScanArgs {
