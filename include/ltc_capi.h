@@ -293,15 +293,19 @@ int ltc_ode_unfold_bwd(const float* v_buffer, const float* w_pos, const float* w
  * whose time axis is parallel, and what turns a layer's outputs into token
  * scores and training losses. Tensors are fp32, bf16 or fp16 (LTC_F32, LTC_BF16,
  * LTC_F16), unit stride along their last dimension, any alignment their type
- * has; states, sums and statistics are fp32. Results are deterministic.
+ * has; states, sums and statistics are fp32. Results are deterministic. A
+ * workspace (256-byte aligned) serves one call at a time: calls on one stream may
+ * share it, calls that may run at once may not. Nothing in it has to be cleared or
+ * kept between calls. Outputs overlap neither inputs nor one another.
  */
 #define LTC_F32 0
 #define LTC_BF16 1
 #define LTC_F16 2
 
 /* Gate forms: a = sigmoid(gate), h = a h + (1 - a) x; a = exp(gate), h = a h + x.
- * exp(gate) over 1 is taken as it is: the product of the decays of up to 256
- * tokens has to stay in fp32's range then. */
+ * exp(gate) over 1 is taken as it is: the product of the decays of any run of a
+ * sequence's tokens has to stay in fp32's range then, and its outputs may be infinite
+ * or NaN where it does not. */
 #define LTC_GATE_BLEND 0
 #define LTC_GATE_DECAY 1
 
@@ -311,7 +315,9 @@ int ltc_ode_unfold_bwd(const float* v_buffer, const float* w_pos, const float* w
  * tokens in all: sequence s is tokens cu_seqlens[s] up to cu_seqlens[s + 1], and
  * may be empty. Tokens outside every sequence give zeros, in out and in the
  * gradients. Boundaries outside 0 ... T or out of order give unspecified results
- * without an access out of range.
+ * without an access out of range. Workgroups hand states on through the workspace;
+ * one whose wait for another outlasts ltc_set_cluster_spin_ticks()'s budget goes on
+ * with NaN.
  *   x            (B,T,H) with element strides sxb, sxt; packed (T,H), stride sxt
  *   gate         likewise; its type is x's or LTC_F32
  *   state        (B,H) fp32 contiguous, or NULL for zero
@@ -490,7 +496,8 @@ int ltc_launch_plan(int B, int T, int D, int H, int ode_unfolds, long long* out,
  */
 int ltc_device_status(int clear);
 
-/* Wait budget of every cluster exchange (and companion wait), in ticks of the GPU's 100 MHz wall
+/* Wait budget of every cluster exchange (and companion wait, and of the gated
+ * scan's waits), in ticks of the GPU's 100 MHz wall
  * clock (default 20000000 = 0.2 s), for calls made after it returns; returns
  * the previous budget, or -1 for a negative argument. A budget of 0 makes
  * every member give up at its first wait: a host-forced failure for tests of

@@ -919,6 +919,7 @@ namespace ltc {
 int host_fail(int code, const std::string& msg) { return fail(code, msg); }
 int host_hip_fail(const char* what, hipError_t e) { return hip_fail(what, e); }
 void host_clear_error() { g_err.clear(); }
+long long host_spin_ticks() { return g_spin.load(std::memory_order_relaxed); }
 hipError_t host_timed(int id, hipError_t (*launch)(void*), void* ctx) {
   return timed(id, nullptr, [&] { return launch(ctx); });
 }

@@ -223,7 +223,9 @@ struct SlotMaps {
 // kScanGroup leaves the map of its group. What enters a tile then comes from the
 // maps of the groups before its own and of the tiles before it in its group, from
 // the tile on that holds the sequence's first token: two hops however long the
-// sequence, and the same order of sums in every run.
+// sequence, and the same order of sums in every run. Every wait is bounded all the
+// same, by the budget of the framework's other waits between workgroups: two calls
+// at once on one workspace end, with NaN.
 // ---------------------------------------------------------------------------
 constexpr unsigned long long kNoWord = ~0ull;
 
@@ -251,11 +253,16 @@ struct Words {
     for (int j = 0; j < N; ++j) m = m || q[j] == kNoWord;
     return m;
   }
-  __device__ __forceinline__ void wait(const unsigned long long* w, unsigned at, unsigned stride, int n) {
-    while (missing()) {
+  // For spin ticks of the wall clock at most. A word that does not come is itself a
+  // map that gives NaN, so what hangs on it is NaN then.
+  __device__ __forceinline__ void wait(const unsigned long long* w, unsigned at, unsigned stride, int n,
+                                       long long spin) {
+    if (!missing()) return;
+    const long long t0 = wall_clock64();
+    do {
       __builtin_amdgcn_s_sleep(1);
       read(w, at, stride, n);
-    }
+    } while (missing() && wall_clock64() - t0 < spin);
   }
   // (A, B) composed with the first n, in their order.
   __device__ __forceinline__ void fold(int n, float& A, float& B) const {
@@ -305,7 +312,7 @@ struct LookBack {
     qt.read(wt, at, p.H, tn);
     qg.read(wg, ag, p.H, gn);
     float a = 1.f, b = 0.f;
-    qt.wait(wt, at, p.H, tn);
+    qt.wait(wt, at, p.H, tn, p.spin);
     qt.fold(tn, a, b);
     ta[part][c] = a;
     tb[part][c] = b;
@@ -322,12 +329,12 @@ struct LookBack {
     }
     a = 1.f;
     b = 0.f;
-    qg.wait(wg, ag, p.H, gn);
+    qg.wait(wg, ag, p.H, gn, p.spin);
     qg.fold(gn, a, b);
     for (int i = kGroups; i < gn; i += kGroups) {
       const unsigned ai = ag + (unsigned)i * p.H;
       qg.read(wg, ai, p.H, gn - i);
-      qg.wait(wg, ai, p.H, gn - i);
+      qg.wait(wg, ai, p.H, gn - i, p.spin);
       qg.fold(gn - i, a, b);
     }
     ga[part][c] = a;
@@ -338,7 +345,8 @@ struct LookBack {
       b = 0.f;
       join(ga, gb, c, a, b);
       join(ta, tb, c, a, b);
-      enter[c] = first < l ? b : 0.f;
+      // without a budget every wait counts as given up
+      enter[c] = first == l ? 0.f : p.spin > 0 ? b : __builtin_nanf("");
     }
     __syncthreads();
   }

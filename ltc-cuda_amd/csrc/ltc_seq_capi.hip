@@ -244,6 +244,7 @@ int ltc_gated_scan_forward(const void* x, long long sxb, long long sxt, const vo
   a.states = sv.states;
   a.words = w.words;
   a.tickets = w.tickets;
+  a.spin = ltc::host_spin_ticks();
   ltc::scan_tiles(x_type, N, H, &a);
   int* marks = save ? sv.marks : w.marks;
   a.cu = cu_seqlens;
@@ -302,6 +303,7 @@ int ltc_gated_scan_backward(const void* x, long long sxb, long long sxt, const v
   a.states = sv.states;
   a.words = w.words;
   a.tickets = w.tickets;
+  a.spin = ltc::host_spin_ticks();
   ltc::scan_tiles(x_type, N, H, &a);
   a.gx = grad_x;
   a.gg = grad_gate;

@@ -45,6 +45,7 @@ struct ScanArgs {
   float* states;     // what enters each tile (ntiles,H); forward: may be null
   unsigned long long* words;  // maps of tiles (ntiles,H), then of groups of tiles
   unsigned* tickets;  // one for each range of channel blocks, every kTicketStride words
+  long long spin;     // wait budget, wall-clock ticks
   void* gx;          // backward (N,H), or null where not wanted
   void* gg;          // backward (N,H), or null
   float* gs;         // backward (B,H), or null
@@ -135,6 +136,7 @@ hipError_t launch_distill_bwd(int x_type, const TokArgs& a, hipStream_t s);
 int host_fail(int code, const std::string& msg);
 int host_hip_fail(const char* what, hipError_t e);
 void host_clear_error();
+long long host_spin_ticks();  // ltc_set_cluster_spin_ticks
 // Runs launch(ctx); while timing is on, its kernels count under `id`.
 hipError_t host_timed(int id, hipError_t (*launch)(void*), void* ctx);
 

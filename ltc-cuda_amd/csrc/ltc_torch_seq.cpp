@@ -6,6 +6,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
@@ -269,6 +270,9 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& state,
   }
   check_device(gate, x, "gate");
   check_device(state, x, "state");
+  // workgroups read x and gate while others write the state
+  at::assert_no_overlap(state, x);
+  at::assert_no_overlap(state, gate);
   TORCH_CHECK(!torch::GradMode::is_enabled() ||
                   !torch::autograd::compute_requires_grad(x, gate, state),
               "ltc_gated_scan_step has no backward: call it under torch.no_grad(), or ltc_gated_scan");

@@ -899,8 +899,9 @@ def ltc_gated_scan(x, gate, state=None, cu_seqlens=None, form="blend"):
     form "blend": a = sigmoid(gate), h_t = a_t h_{t-1} + (1 - a_t) x_t, the update
     of an LTC neuron without recurrent synapses (a = cm / (cm + conductances), x
     the potential they drive it to). form "decay": a = exp(gate), h_t = a_t h_{t-1}
-    + x_t; gates over 0 are taken as they are, and overflow where their product
-    over 256 tokens does.
+    + x_t; gates over 0 are taken as they are: where the product of the decays of
+    some run of a sequence's tokens leaves float32's range, results may be infinite
+    or NaN.
 
     x       (B, T, H), float32, bfloat16 or float16; with cu_seqlens (tokens, H)
     gate    x's shape; its type is x's or float32
