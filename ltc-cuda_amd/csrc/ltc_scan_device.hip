@@ -32,16 +32,26 @@ constexpr int kMarkNone = -1, kMarkStart = 1, kMarkEnd = 2;
 // a and 1 - a (decay: 1), each to its own relative precision: with e = exp(-g),
 // a = 1 / (1 + e) and 1 - a = e a. e is kept below 2^126, where a is 2^-126 and
 // 1 - a is 1; `minimum` passes a NaN on.
+// exp_of is e, or in the other form a itself, from which gate_from goes on.
 template <int FORM>
-__device__ __forceinline__ void gate_of(float g, float& a, float& na) {
+__device__ __forceinline__ float exp_of(float g) {
+  return FORM == LTC_GATE_BLEND
+             ? __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(g * -kLog2e, 126.f))
+             : __builtin_amdgcn_exp2f(g * kLog2e);
+}
+template <int FORM>
+__device__ __forceinline__ void gate_from(float e, float& a, float& na) {
   if constexpr (FORM == LTC_GATE_BLEND) {
-    const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(g * -kLog2e, 126.f));
     a = __builtin_amdgcn_rcpf(1.f + e);
     na = e * a;
   } else {
-    a = __builtin_amdgcn_exp2f(g * kLog2e);
+    a = e;
     na = 1.f;
   }
+}
+template <int FORM>
+__device__ __forceinline__ void gate_of(float g, float& a, float& na) {
+  gate_from<FORM>(exp_of<FORM>(g), a, na);
 }
 
 // A thread's tokens: bit i of the masks is token i. Tokens outside all sequences
@@ -400,6 +410,13 @@ __device__ __forceinline__ void forget(Vec<T, V> (&r)[LT]) {
 #pragma unroll
     for (int j = 0; j < Vec<T, V>::kWords; ++j) asm volatile("" : "+v"(r[i].w[j]));
 }
+template <int V, int LT>
+__device__ __forceinline__ void forget(float (&r)[LT][V]) {
+#pragma unroll
+  for (int i = 0; i < LT; ++i)
+#pragma unroll
+    for (int v = 0; v < V; ++v) asm volatile("" : "+v"(r[i][v]));
+}
 
 // LOOK: tiles hand states on; else every tile begins with a sequence, or is the
 // only one.
@@ -506,7 +523,10 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 4) void scan_fwd_kernel(ScanArgs
 // Backward: the carry from token t + 1 to t is a_{t+1} d_{t+1}, nothing across
 // sequences. The states are run again from what entered the tile. Gates are formed
 // three times (for the maps, the states, the gradients): kept, they take 64
-// registers more, which spill.
+// registers more, which spill. Of 16-bit inputs their exponentials are kept, in 16
+// registers more: the kernel is bound by its arithmetic there as much as by its bytes
+// (B8 T4096 H2048 bf16 175 us and 185, 3.8 TB/s). In fp32, with half the arithmetic to
+// a byte, it runs faster without (H1024 159 us and 173, 4.2 TB/s).
 template <class T, class G, int FORM, bool PACKED, bool LOOK>
 __global__ __launch_bounds__(Scan<T>::kThreads, 3) void scan_bwd_kernel(ScanArgs p) {
   constexpr int V = Scan<T>::V, CB = Scan<T>::CB, LT = kScanTokens;
@@ -521,6 +541,12 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 3) void scan_bwd_kernel(ScanArgs
   const Tokens<LT> k = tokens_of<LT, PACKED>(p, tile * kScanTile + slot * LT);
   Vec<T, V> x[LT], go[LT];
   Vec<G, V> g[LT];
+  constexpr bool KEEP = sizeof(T) == 2;
+  float ex[LT][V];  // KEEP: exp_of the gates, else the gates
+  auto gate = [&](int i, int v, float& a, float& na) {
+    if constexpr (KEEP) gate_from<FORM>(ex[i][v], a, na);
+    else gate_of<FORM>(ex[i][v], a, na);
+  };
   load_tokens<T, V, LT, PACKED>(p.x, p.sxb, p.sxt, p, k, ch, n, x);
   load_tokens<G, V, LT, PACKED>(p.g, p.sgb, p.sgt, p, k, ch, n, g);
   load_tokens<T, V, LT, PACKED>(p.go, p.sob, p.sot, p, k, ch, n, go);
@@ -545,7 +571,8 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 3) void scan_bwd_kernel(ScanArgs
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         float na;
-        gate_of<FORM>(g[i].get(v), a[i][v], na);
+        ex[i][v] = KEEP ? exp_of<FORM>(g[i].get(v)) : g[i].get(v);
+        gate(i, v, a[i][v], na);
         const float xv = x[i].get(v);
         A[v] *= a[i][v];
         B[v] = fmaf(a[i][v], B[v], FORM == LTC_GATE_BLEND ? na * xv : xv);
@@ -587,7 +614,7 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 3) void scan_bwd_kernel(ScanArgs
     lb.run(p, l, first, c0, ta, tb);
   }
   forget(x);
-  forget(g);
+  forget(ex);
   forget(go);
   if (n <= 0 || k.t0 >= p.N) return;
   float hp[LT][V], e[V];  // state before token i, carry into it
@@ -608,14 +635,14 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 3) void scan_bwd_kernel(ScanArgs
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         float a, na;
-        gate_of<FORM>(g[i].get(v), a, na);
+        gate(i, v, a, na);
         const float xv = x[i].get(v);
         hp[i][v] = h[v];
         h[v] = fmaf(a, h[v], FORM == LTC_GATE_BLEND ? na * xv : xv);
       }
     }
   }
-  forget(g);
+  forget(ex);
   long long at = (long long)k.t0 * p.H + ch + (LT - 1) * (long long)p.H;
 #pragma unroll
   for (int i = LT - 1; i >= 0; --i, at -= p.H) {
@@ -631,7 +658,7 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 3) void scan_bwd_kernel(ScanArgs
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       float a, na;
-      gate_of<FORM>(g[i].get(v), a, na);
+      gate(i, v, a, na);
       const float d = o[v] + e[v];
       e[v] = ds[v] = a * d;
       if constexpr (FORM == LTC_GATE_BLEND) {
