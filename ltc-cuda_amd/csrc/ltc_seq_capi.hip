@@ -392,6 +392,7 @@ int ltc_token_logprobs_backward(const void* logits, long long sl, const void* id
   a.ge = grad_entropy;
   a.sge = sen;
   a.gx = grad_logits;
+  ltc::tok_split_bwd(N, V, type_bytes(logits_type), kMaxGroups, &a.nsplit, &a.seg);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const hipError_t e =
       host_timed(ltc::K_LOGPROBS_BWD, [&] { return ltc::launch_logprobs_bwd(logits_type, a, s); });
@@ -453,6 +454,7 @@ int ltc_top_distill_backward(const void* logits, long long sl, const void* teach
   a.gp = grad_loss;
   a.sgp = sgl;
   a.gx = grad_logits;
+  ltc::tok_split_bwd(N, V, type_bytes(logits_type), kMaxGroups, &a.nsplit, &a.seg);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const hipError_t e =
       host_timed(ltc::K_DISTILL_BWD, [&] { return ltc::launch_distill_bwd(logits_type, a, s); });

@@ -125,6 +125,8 @@ struct TokArgs {
 
 // Logits per workgroup and workgroups per row.
 void tok_split(long long N, int V, int elem_bytes, int top, int* nsplit, int* seg);
+// The same of the backward, which needs no join; `most` workgroups in all.
+void tok_split_bwd(long long N, int V, int elem_bytes, long long most, int* nsplit, int* seg);
 hipError_t launch_logprobs_fwd(int x_type, const TokArgs& a, hipStream_t s);
 hipError_t launch_logprobs_bwd(int x_type, const TokArgs& a, hipStream_t s);
 hipError_t launch_distill_fwd(int x_type, const TokArgs& a, hipStream_t s);

@@ -167,3 +167,28 @@ def test_two_streams_at_once():
     for res in got:
         for a, b in zip(res, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+@pytest.mark.parametrize("N,V,K", [(1030, 20011, 64), (3, 20011, 1000), (1025, 5000, 1), (2, 70, 1024)])
+def test_distill_entries_over_segments(N, V, K, dtype):
+    """Entries that come several times, at a gradient's segments' edges, missing ones
+    between them; the same gradient each time."""
+    g = torch.Generator().manual_seed(N + K)
+    x, t = torch.randn(N, V, generator=g).to(dtype), torch.randn(N, K, generator=g)
+    ids = torch.randint(0, V, (N, K), generator=g)
+    edges = torch.tensor([0, 2047, 2048, 4095, 4096, V - 1]).clamp(max=V - 1)
+    some = torch.rand(N, K, generator=g)
+    ids = torch.where(some < 0.3, edges[torch.randint(0, 6, (N, K), generator=g)], ids)
+    ids = torch.where(some > 0.9, -torch.ones_like(ids), ids)
+    gl = torch.rand(N, generator=g)
+    leaf = x.to(DEV).requires_grad_(True)
+    grads = []
+    for _ in range(2):
+        loss = ltc_cuda.ltc_top_distill(leaf, t.to(DEV), ids.to(DEV), temperature=2.0)
+        grads += torch.autograd.grad(loss, [leaf], [gl.to(DEV)])
+    assert torch.equal(*grads)
+    rows = sorted({0, 1, N - 1})
+    val, tol = R.distill(x[rows], t[rows], ids[rows], 2.0, gl[rows])
+    R.close(loss.detach().cpu()[rows], val["loss"], tol["loss"], "loss")
+    R.close(grads[0].cpu()[rows], val["gx"], tol["gx"], "gx")
