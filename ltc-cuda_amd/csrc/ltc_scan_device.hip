@@ -419,7 +419,9 @@ __device__ __forceinline__ void forget(float (&r)[LT][V]) {
 }
 
 // LOOK: tiles hand states on; else every tile begins with a sequence, or is the
-// only one.
+// only one. B8 T4096 H2048 bf16 takes 96 us, 4.2 TB/s, and without handing on (T128) 77,
+// 5.2: bound by bytes, arithmetic (formed twice, the gates cost bf16 9 us more) and the
+// wait. The four workgroups that a CU holds cover one another's waits.
 template <class T, class G, int FORM, bool PACKED, bool LOOK>
 __global__ __launch_bounds__(Scan<T>::kThreads, 4) void scan_fwd_kernel(ScanArgs p) {
   constexpr int V = Scan<T>::V, CB = Scan<T>::CB, LT = kScanTokens;
@@ -727,7 +729,8 @@ constexpr int kStepThreads = 256, kStepChannels = 4;
 // One token of each row, its state updated in place. A row whose slot an
 // earlier row names too is left to that row, which takes the rows of its slot
 // one after the other, as tokens of one stream. Bound by latency: the loads are
-// under way before the workgroup has looked through the slots for its own.
+// under way before the workgroup has looked through the slots for its own (one row of
+// 64 1.5 us, 256 rows of 2048 in a pool 4.0).
 template <class T, class G, int FORM>
 __global__ __launch_bounds__(kStepThreads) void scan_step_kernel(StepArgs p) {
   constexpr int V = kStepChannels;

