@@ -264,16 +264,18 @@ struct Words {
     for (int j = 0; j < N; ++j) m = m || q[j] == kNoWord;
     return m;
   }
-  // For spin ticks of the wall clock at most. A word that does not come is itself a
-  // map that gives NaN, so what hangs on it is NaN then.
+  // For spin ticks of the wall clock, and kScanPolls reads (the clock goes on while a
+  // process is put aside, its workgroups together). A word that does not come is itself
+  // a map that gives NaN, so what hangs on it is NaN then.
   __device__ __forceinline__ void wait(const unsigned long long* w, unsigned at, unsigned stride, int n,
                                        long long spin) {
     if (!missing()) return;
     const long long t0 = wall_clock64();
+    int polls = 0;
     do {
       __builtin_amdgcn_s_sleep(1);
       read(w, at, stride, n);
-    } while (missing() && wall_clock64() - t0 < spin);
+    } while (missing() && (++polls < kScanPolls || wall_clock64() - t0 < spin));
   }
   // (A, B) composed with the first n, in their order.
   __device__ __forceinline__ void fold(int n, float& A, float& B) const {

@@ -22,6 +22,8 @@ constexpr int kScanTokens = 4;
 constexpr int kScanTile = kScanSlots * kScanTokens;
 // Tiles whose maps are composed into one.
 constexpr int kScanGroup = 16;
+// Reads of a word before a wait for it may be given up: some milliseconds.
+constexpr int kScanPolls = 4096;
 // Ranges of channel blocks, and the words between their counters.
 constexpr int kScanRanges = 7;
 constexpr int kTicketStride = 64;
