@@ -296,10 +296,13 @@ struct LookBack {
   static constexpr int kTiles = kScanGroup / kParts;  // a part's share of a group
   static constexpr int kGroups = 4;  // words of a batch: more cost registers, and those spill
   float ta[kParts][CB], tb[kParts][CB], ga[kParts][CB], gb[kParts][CB];
-  float enter[CB];
+  // The workgroup's number in order, before run(); what enters the tile, after it. No
+  // places of their own: so four workgroups of the 16-bit backward fill a CU's 160 KiB.
+  __device__ __forceinline__ unsigned& ticket() { return *reinterpret_cast<unsigned*>(&ta[0][0]); }
+  __device__ __forceinline__ float& enter(int c) { return ga[0][c]; }
 
   // Leaves the tile's map (A, B: valid in threads below CB) and what enters the
-  // tile, in enter[]. `first`: the tile from which on maps count, l for none.
+  // tile, in enter(). `first`: the tile from which on maps count, l for none.
   __device__ __forceinline__ void run(const ScanArgs& p, int l, int first, int c0, float A, float B) {
     const int c = threadIdx.x % CB, part = threadIdx.x / CB;
     const int ch = Scan<T>::channel(c);
@@ -361,7 +364,7 @@ struct LookBack {
       join(ga, gb, c, a, b);
       join(ta, tb, c, a, b);
       // without a budget every wait counts as given up
-      enter[c] = first == l ? 0.f : p.spin > 0 ? b : __builtin_nanf("");
+      enter(c) = first == l ? 0.f : p.spin > 0 ? b : __builtin_nanf("");
     }
     __syncthreads();
   }
@@ -387,17 +390,16 @@ struct NoLookBack {};
 // ranges, not eight: with one to an XCD each XCD keeps to the same few memory channels
 // where rows are powers of two (H2048 forward 95 us and 103, one tile a sequence 76
 // and 83).
-template <bool LOOK>
-__device__ __forceinline__ void take_tile(const ScanArgs& p, int& tile, int& cblock) {
+template <bool LOOK, class LB>
+__device__ __forceinline__ void take_tile(const ScanArgs& p, LB& lb, int& tile, int& cblock) {
   const unsigned range = blockIdx.x % p.ranges;
   unsigned t = blockIdx.x / p.ranges;
   if constexpr (LOOK) {
-    __shared__ unsigned ticket;
     if (threadIdx.x == 0)
-      ticket = __hip_atomic_fetch_add(p.tickets + range * kTicketStride, 1u, __ATOMIC_RELAXED,
-                                      __HIP_MEMORY_SCOPE_AGENT);
+      lb.ticket() = __hip_atomic_fetch_add(p.tickets + range * kTicketStride, 1u, __ATOMIC_RELAXED,
+                                           __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    t = ticket;
+    t = lb.ticket();
   }
   tile = t / p.per;
   cblock = range * p.per + t % p.per;
@@ -431,7 +433,7 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 4) void scan_fwd_kernel(ScanArgs
   __shared__ typename std::conditional<LOOK, LookBack<T>, NoLookBack>::type lb;
   const int c = threadIdx.x % Scan<T>::kLanes, slot = threadIdx.x / Scan<T>::kLanes;
   int tile, cblock;
-  take_tile<LOOK>(p, tile, cblock);
+  take_tile<LOOK>(p, lb, tile, cblock);
   if (cblock >= p.cblocks) return;  // the last range may be short
   const int c0 = cblock * CB, ch = c0 + c * V, n = p.H - ch;
   const Tokens<LT> k = tokens_of<LT, PACKED>(p, tile * kScanTile + slot * LT);
@@ -492,7 +494,7 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 4) void scan_fwd_kernel(ScanArgs
   for (int v = 0; v < V; ++v) {
     const int at = Scan<T>::place(c, v);
     float enter = 0.f;
-    if constexpr (LOOK) enter = lb.enter[at];
+    if constexpr (LOOK) enter = lb.enter(at);
     h[v] = sm.enter(slot, at, enter);
   }
   // the backward starts its tiles from these
@@ -531,14 +533,17 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 4) void scan_fwd_kernel(ScanArgs
 // registers more: the kernel is bound by its arithmetic there as much as by its bytes
 // (B8 T4096 H2048 bf16 175 us and 185, 3.8 TB/s). In fp32, with half the arithmetic to
 // a byte, it runs faster without (H1024 159 us and 173, 4.2 TB/s).
+// Decays need fewer registers: four workgroups to a CU for three (B8 T4096 H2048 bf16
+// 150 us and 161, packed the same).
 template <class T, class G, int FORM, bool PACKED, bool LOOK>
-__global__ __launch_bounds__(Scan<T>::kThreads, 3) void scan_bwd_kernel(ScanArgs p) {
+__global__ __launch_bounds__(Scan<T>::kThreads, sizeof(T) == 2 && FORM == LTC_GATE_DECAY ? 4 : 3)
+    void scan_bwd_kernel(ScanArgs p) {
   constexpr int V = Scan<T>::V, CB = Scan<T>::CB, LT = kScanTokens;
   __shared__ SlotMaps<T> sf, sr;
   __shared__ typename std::conditional<LOOK, LookBack<T>, NoLookBack>::type lb;
   const int c = threadIdx.x % Scan<T>::kLanes, slot = threadIdx.x / Scan<T>::kLanes;
   int l, cblock;
-  take_tile<LOOK>(p, l, cblock);
+  take_tile<LOOK>(p, lb, l, cblock);
   if (cblock >= p.cblocks) return;  // the last range may be short
   const int tile = (int)p.ntiles - 1 - l;
   const int c0 = cblock * CB, ch = c0 + c * V, n = p.H - ch;
@@ -630,7 +635,7 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 3) void scan_bwd_kernel(ScanArgs
       const int at = Scan<T>::place(c, v);
       h[v] = sf.enter(slot, at, q.get(v));
       float enter = 0.f;
-      if constexpr (LOOK) enter = lb.enter[at];
+      if constexpr (LOOK) enter = lb.enter(at);
       e[v] = sr.enter(kScanSlots - 1 - slot, at, enter);
     }
 #pragma unroll
