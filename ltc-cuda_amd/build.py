@@ -35,7 +35,7 @@ def source_files() -> list:
     inc = os.path.join(os.path.dirname(HERE), "include", "ltc_capi.h")
     return [os.path.join(CSRC, s) for s in SOURCES] + [
         os.path.join(CSRC, "ltc_internal.h"), os.path.join(CSRC, "ltc_seq_internal.h"),
-        os.path.join(CSRC, "ltc_vec.h"),
+        os.path.join(CSRC, "ltc_vec.h"), os.path.join(CSRC, "ltc_torch_checks.h"),
         *[os.path.join(CSRC, s) for s in EXT_SOURCES], inc]
 
 
