@@ -9,6 +9,7 @@ import torch
 import torch.autograd.forward_ad as fw
 from torch.fx.experimental.proxy_tensor import make_fx
 
+import ltc
 import ltc_cuda
 
 GPU = pytest.param("cuda", marks=pytest.mark.gpu)
@@ -32,7 +33,21 @@ def _calls(ext, device):
     x = torch.randn(2, 3, 4, device=device)
     y, st = x[:, 0].contiguous(), torch.randn(2, 4, device=device)
     ids = torch.zeros(2, 3, dtype=torch.long, device=device)
+    D, H = 4, 4
+    m = ltc.TrueLiquidTimeConstant(D, H).to(device)
+    named = {**dict(m.named_parameters()), **dict(m.named_buffers())}
+    leaves = [named[n].detach() for n in ltc_cuda.MODULE_LEAVES]
+
+    def layer(a, i):
+        args = [x, st, *leaves]
+        args[i] = a
+        return ext.module_apply(args[0], args[1], args[2:], 0.1, 2, 1e-8, 1e-5)[0]
+
     return [
+        ("ltc_module_forward", lambda a: layer(a, 0), x),
+        ("ltc_module_forward", lambda a: layer(a, 1), st),
+        ("ltc_module_forward", lambda a: layer(a, 2), leaves[0]),
+        ("ltc_module_forward", lambda a: layer(a, 18), leaves[16]),
         ("ltc_gated_scan", lambda a: ext.gated_scan(a, x, None, None, 0)[0], x),
         ("ltc_gated_scan", lambda a: ext.gated_scan(x, a, st, None, 1)[0], x),
         ("ltc_gated_scan", lambda a: ext.gated_scan(x, x, a, None, 0)[1], st),
