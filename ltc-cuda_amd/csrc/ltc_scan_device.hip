@@ -266,16 +266,17 @@ struct Words {
   }
   // For spin ticks of the wall clock, and kScanPolls reads (the clock goes on while a
   // process is put aside, its workgroups together). A word that does not come is itself
-  // a map that gives NaN, so what hangs on it is NaN then.
+  // a map that gives NaN, so what hangs on it is NaN then. The wave waits as one: lane by
+  // lane, the loop's own state costs the packed decays' backward two registers, which spill.
   __device__ __forceinline__ void wait(const unsigned long long* w, unsigned at, unsigned stride, int n,
                                        long long spin) {
-    if (!missing()) return;
+    if (!__any(missing())) return;
     const long long t0 = wall_clock64();
     int polls = 0;
     do {
       __builtin_amdgcn_s_sleep(1);
       read(w, at, stride, n);
-    } while (missing() && (++polls < kScanPolls || wall_clock64() - t0 < spin));
+    } while (__any(missing()) && (++polls < kScanPolls || wall_clock64() - t0 < spin));
   }
   // (A, B) composed with the first n, in their order.
   __device__ __forceinline__ void fold(int n, float& A, float& B) const {
@@ -533,8 +534,9 @@ __global__ __launch_bounds__(Scan<T>::kThreads, 4) void scan_fwd_kernel(ScanArgs
 // registers more: the kernel is bound by its arithmetic there as much as by its bytes
 // (B8 T4096 H2048 bf16 175 us and 185, 3.8 TB/s). In fp32, with half the arithmetic to
 // a byte, it runs faster without (H1024 159 us and 173, 4.2 TB/s).
-// Decays need fewer registers: four workgroups to a CU for three (B8 T4096 H2048 bf16
-// 150 us and 161, packed the same).
+// Decays need fewer registers, 128 of them: four workgroups to a CU for three (with the
+// preparation, B8 T4096 H2048 bf16 140 us and 152; 30011 tokens in 37 sequences, H1000
+// bf16, fp32 gates 137 and 141).
 template <class T, class G, int FORM, bool PACKED, bool LOOK>
 __global__ __launch_bounds__(Scan<T>::kThreads, sizeof(T) == 2 && FORM == LTC_GATE_DECAY ? 4 : 3)
     void scan_bwd_kernel(ScanArgs p) {
