@@ -317,7 +317,7 @@ int ltc_ode_unfold_bwd(const float* v_buffer, const float* w_pos, const float* w
  * gradients. Boundaries outside 0 ... T or out of order give unspecified results
  * without an access out of range. Workgroups hand states on through the workspace;
  * one whose wait for another outlasts ltc_set_cluster_spin_ticks()'s budget goes on
- * with NaN.
+ * with NaN, and a sticky flag of the device is raised (ltc_scan_status).
  *   x            (B,T,H) with element strides sxb, sxt; packed (T,H), stride sxt
  *   gate         likewise; its type is x's or LTC_F32
  *   state        (B,H) fp32 contiguous, or NULL for zero
@@ -348,6 +348,14 @@ int ltc_gated_scan_backward(const void* x, long long sxb, long long sxt, const v
                             long long sob, long long sot, const float* grad_state_final,
                             void* grad_x, void* grad_gate, float* grad_state, void* workspace,
                             long long workspace_bytes, void* stream);
+
+/*
+ * Whether a scan on the current device has given up a wait, forward or backward: waits
+ * for the device and returns LTC_EHIP with a message if so, clearing the flag when
+ * `clear` is nonzero. ltc_device_status() reports the other kernels' waits, not these.
+ * As that, not to be called under graph capture.
+ */
+int ltc_scan_status(int clear);
 
 /*
  * One token of B streams: out[b] and the stream's new state, written over the old.
@@ -492,6 +500,7 @@ int ltc_launch_plan(int B, int T, int D, int H, int ode_unfolds, long long* out,
  * ltc_device_status() waits for the current device, returns LTC_EHIP with a
  * message when the flag is raised, and clears it when `clear` is nonzero.
  * It synchronises the device, so it must not be called under graph capture.
+ * The gated scan's waits have a flag of their own (ltc_scan_status()).
  * No counterpart in the reference, whose kernels have no inter-block waits.
  */
 int ltc_device_status(int clear);

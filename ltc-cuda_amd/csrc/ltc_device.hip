@@ -6554,14 +6554,18 @@ hipError_t launch_fill(const FillList& fl, hipStream_t s) {
 }
 
 hipError_t device_fault(int* value, bool clear) {
+  return read_flag(&g_fault, value, clear);
+}
+
+hipError_t read_flag(const void* symbol, int* value, bool clear) {
   hipError_t e = hipDeviceSynchronize();
   if (e != hipSuccess) return e;
   int v = 0;
-  e = hipMemcpyFromSymbol(&v, HIP_SYMBOL(g_fault), sizeof(int), 0, hipMemcpyDeviceToHost);
+  e = hipMemcpyFromSymbol(&v, symbol, sizeof(int), 0, hipMemcpyDeviceToHost);
   if (e != hipSuccess) return e;
   if (clear && v != 0) {
     const int zero = 0;
-    e = hipMemcpyToSymbol(HIP_SYMBOL(g_fault), &zero, sizeof(int), 0, hipMemcpyHostToDevice);
+    e = hipMemcpyToSymbol(symbol, &zero, sizeof(int), 0, hipMemcpyHostToDevice);
     if (e != hipSuccess) return e;
   }
   *value = v;

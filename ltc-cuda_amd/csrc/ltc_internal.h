@@ -352,6 +352,8 @@ inline void fill_add(FillList& fl, float* dst, const float* src, long long n) {
 // The current device's sticky fault flag: reads it (after waiting for the
 // device) and clears it when `clear` is set. Returns the HIP status.
 hipError_t device_fault(int* value, bool clear);
+// The same of any flag, a __device__ int.
+hipError_t read_flag(const void* symbol, int* value, bool clear);
 // Exchange words of one cluster launch (forward / chain).
 inline long long cluster_words(const Plan& p) {
   if (p.rf.CP > 0) return 2LL * p.rf.NCL * p.rf.CP * p.rf.NB * p.rf.JW;

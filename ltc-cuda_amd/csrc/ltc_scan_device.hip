@@ -236,9 +236,16 @@ struct SlotMaps {
 // behind that, from the tiles' alone: two hops however long the sequence, and the same
 // order of sums in every run. Every wait is bounded all the
 // same, by the budget of the framework's other waits between workgroups: two calls
-// at once on one workspace end, with NaN.
+// at once on one workspace end, with NaN and the flag raised.
 // ---------------------------------------------------------------------------
 constexpr unsigned long long kNoWord = ~0ull;
+
+// The device's sticky flag of waits that were given up, read and cleared by the
+// host (scan_fault).
+__device__ int g_scan_fault;
+__device__ __forceinline__ void gave_up() {
+  __hip_atomic_store(&g_scan_fault, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 
 __device__ __forceinline__ void put_word(unsigned long long* w, float A, float B) {
   unsigned a = __float_as_uint(A);
@@ -277,6 +284,7 @@ struct Words {
       __builtin_amdgcn_s_sleep(1);
       read(w, at, stride, n);
     } while (__any(missing()) && (++polls < kScanPolls || wall_clock64() - t0 < spin));
+    if (__any(missing())) gave_up();
   }
   // (A, B) composed with the first n, in their order.
   __device__ __forceinline__ void fold(int n, float& A, float& B) const {
@@ -365,6 +373,7 @@ struct LookBack {
       join(ga, gb, c, a, b);
       join(ta, tb, c, a, b);
       // without a budget every wait counts as given up
+      if (first != l && p.spin <= 0) gave_up();
       enter(c) = first == l ? 0.f : p.spin > 0 ? b : __builtin_nanf("");
     }
     __syncthreads();
@@ -876,6 +885,10 @@ hipError_t launch_scan(const ScanTypes& ty, const ScanArgs& a, bool bwd, hipStre
       return hipGetLastError();
     });
   });
+}
+
+hipError_t scan_fault(int* value, bool clear) {
+  return read_flag(&g_scan_fault, value, clear);
 }
 
 hipError_t launch_scan_step(int x_type, int g_type, int form, const StepArgs& a, hipStream_t s) {

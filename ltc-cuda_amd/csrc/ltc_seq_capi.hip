@@ -320,6 +320,19 @@ int ltc_gated_scan_backward(const void* x, long long sxb, long long sxt, const v
   return e == hipSuccess ? LTC_OK : host_hip_fail("gated scan backward launch", e);
 }
 
+int ltc_scan_status(int clear) {
+  host_clear_error();
+  int v = 0;
+  const hipError_t e = ltc::scan_fault(&v, clear != 0);
+  if (e != hipSuccess) return host_hip_fail("scan status read", e);
+  if (v != 0)
+    return host_fail(LTC_EHIP,
+                     "a gated scan on this device gave up waiting for a state that another of its "
+                     "workgroups hands on (the budget ran out, or two calls at once shared a "
+                     "workspace); what comes from that state is NaN");
+  return LTC_OK;
+}
+
 int ltc_gated_scan_step(const void* x, long long sxb, const void* gate, long long sgb, float* state,
                         long long ssp, const int* slots, int x_type, int gate_type, int form, int B, int H,
                         int P, void* out, void* stream) {

@@ -84,6 +84,8 @@ struct StepArgs {
   int B, H, P;
   void* out;
 };
+// The current device's flag of scans that gave up a wait, as device_fault().
+hipError_t scan_fault(int* value, bool clear);
 hipError_t launch_scan_step(int x_type, int g_type, int form, const StepArgs& a, hipStream_t s);
 
 // ---------------------------------------------------------------------------

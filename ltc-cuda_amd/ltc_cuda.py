@@ -72,7 +72,7 @@ class CApi:
         "ltc_full_forward_noalloc", "ltc_device_status", "ltc_set_cluster_spin_ticks",
         "ltc_gated_scan_saved_floats", "ltc_gated_scan_fwd_workspace_bytes",
         "ltc_gated_scan_bwd_workspace_bytes", "ltc_gated_scan_forward",
-        "ltc_gated_scan_backward", "ltc_gated_scan_step",
+        "ltc_gated_scan_backward", "ltc_scan_status", "ltc_gated_scan_step",
         "ltc_token_logprobs_workspace_bytes", "ltc_token_logprobs_forward",
         "ltc_token_logprobs_backward", "ltc_top_distill_workspace_bytes",
         "ltc_top_distill_forward", "ltc_top_distill_backward",
@@ -192,6 +192,8 @@ class CApi:
         lib.ltc_top_distill_backward.restype = _int
         lib.ltc_top_distill_backward.argtypes = (
             _dist + [_f32p, _f32p, _i64, _f32p, ctypes.c_void_p])
+        lib.ltc_scan_status.restype = _int
+        lib.ltc_scan_status.argtypes = [_int]
         lib.ltc_device_status.restype = _int
         lib.ltc_device_status.argtypes = [_int]
         lib.ltc_set_cluster_spin_ticks.restype = _i64
@@ -235,6 +237,11 @@ class CApi:
         (its outputs were set to NaN); waits for the device. Clears the flag
         unless clear is False."""
         self.check(self.lib.ltc_device_status(1 if clear else 0), "ltc_device_status")
+
+    def scan_status(self, clear: bool = True) -> None:
+        """The same of gated scans: what came from a state that was waited for in
+        vain is NaN."""
+        self.check(self.lib.ltc_scan_status(1 if clear else 0), "ltc_scan_status")
 
     def last_error(self) -> str:
         return self.lib.ltc_last_error().decode(errors="replace")
@@ -786,8 +793,12 @@ def device_status(clear: bool = True) -> None:
     results and nothing is raised), or the companion workgroups of a module backward with one batch
     row per workgroup (the sensory and LayerNorm companions at H <= 64, the
     recurrent-gradient and sensory companions at 64 < H <= 128). The outputs
-    of that call were set to NaN. Synchronises the device."""
-    require_kernels().capi.device_status(clear)
+    of that call were set to NaN. Then the same of ltc_gated_scan, where only
+    what comes from the missing state is NaN (a call that raises for the former
+    leaves this to the next). Synchronises the device."""
+    capi = require_kernels().capi
+    capi.device_status(clear)
+    capi.scan_status(clear)
 
 
 class LTCCudaForward(torch.autograd.Function):
