@@ -4,6 +4,7 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
 #include <ATen/MemoryOverlap.h>
@@ -14,6 +15,8 @@
 
 #include <cstdint>
 #include <limits>
+#include <unordered_set>
+#include <vector>
 
 #include "../../include/ltc_capi.h"
 #include "ltc_torch_checks.h"
@@ -86,20 +89,35 @@ variable_list first_order(variable_list&& g, const char* name) {
 }
 
 // A leaf's gradient accumulator belongs to the stream it was made on, and lives as
-// long as any autograd graph of the leaf. If that is an eager graph, autograd makes
-// the accumulator's stream (the default one, as a rule) wait for the stream under
-// capture as soon as this node returns its gradient, and the end of the capture then
-// takes the process down. So that case is an error here.
+// long as any autograd graph of the leaf. If that is an eager graph of the default
+// stream, autograd makes that stream wait for the one under capture as soon as a node
+// returns the gradient to the accumulator, and the end of the capture then takes the
+// process down. So that case is an error here, for all that the pass will reach from
+// this node on (a module's parameters lie behind others). Other streams can join a
+// capture, and do.
 void check_capture(const Node& node, const Tensor& like) {
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-  const c10::Stream now =
-      c10::impl::VirtualGuardImpl(like.device().type()).getStream(like.device());
-  for (const auto& e : node.next_edges()) {
-    if (!e.is_valid()) continue;
-    const auto s = e.function->stream();
-    TORCH_CHECK(!s.has_value() || *s == now, "a backward pass of ", node.name(),
-                " cannot be captured into a graph while an autograd graph of the same tensors made on "
-                "another stream is alive: drop its outputs first");
+  const c10::Stream eager =
+      c10::impl::VirtualGuardImpl(like.device().type()).getDefaultStream(like.device());
+  // what the pass runs; empty: everything
+  const auto* runs = torch::autograd::get_current_graph_task_exec_info();
+  std::unordered_set<const Node*> seen;
+  std::vector<const Node*> todo{&node};
+  while (!todo.empty()) {
+    const Node* n = todo.back();
+    todo.pop_back();
+    for (const auto& e : n->next_edges()) {
+      if (!e.is_valid() || !seen.insert(e.function.get()).second) continue;
+      if (runs != nullptr && !runs->empty()) {
+        const auto it = runs->find(e.function.get());
+        if (it == runs->end() || !it->second.should_execute()) continue;
+      }
+      const auto s = e.function->stream();
+      TORCH_CHECK(!s.has_value() || s->id() != eager.id(), "a backward pass of ", node.name(),
+                  " cannot be captured into a graph while an autograd graph of the same tensors made on "
+                  "the default stream is alive: drop its outputs first");
+      todo.push_back(e.function.get());
+    }
   }
 }
 
