@@ -13,6 +13,7 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <limits>
 #include <unordered_set>
@@ -262,6 +263,29 @@ std::vector<Tensor> gated_scan(const Tensor& x, const Tensor& gate, const OptTen
   return {out, hf};
 }
 
+// Whether the rows of two matrices of unit stride share a byte. The rows of `table` lie
+// apart from one another, those of t anyhow: of the table's rows that begin before the
+// end of a row of t, the last one reaches furthest.
+bool rows_meet(const Tensor& t, const Tensor& table) {
+  if (t.numel() == 0 || table.numel() == 0) return false;
+  const auto row_bytes = [](const Tensor& q) { return q.size(1) * q.element_size(); };
+  const auto pitch = [](const Tensor& q) { return q.size(0) > 1 ? q.stride(0) * q.element_size() : 0; };
+  const int64_t n = t.size(0), rows = table.size(0), width = row_bytes(table), step = pitch(table);
+  // t's rows as distances from the table's beginning
+  const int64_t begin = (int64_t)(reinterpret_cast<uintptr_t>(t.data_ptr()) -
+                                  reinterpret_cast<uintptr_t>(table.data_ptr()));
+  const auto meets = [&](int64_t lo) {
+    const int64_t hi = lo + row_bytes(t);
+    if (hi <= 0 || lo >= (rows - 1) * step + width) return false;
+    const int64_t r = step > 0 ? std::min((hi - 1) / step, rows - 1) : 0;
+    return r * step + width > lo;
+  };
+  if (begin + (n - 1) * pitch(t) + row_bytes(t) <= 0 || begin >= (rows - 1) * step + width) return false;
+  for (int64_t i = 0; i < n; ++i)
+    if (meets(begin + i * pitch(t))) return true;
+  return false;
+}
+
 Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& state, const OptTensor& slots_opt,
                        int64_t form) {
   check_modes("ltc_gated_scan_step", {x, gate, state});
@@ -303,6 +327,9 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& state,
   {
     at::AutoDispatchBelowADInplaceOrView guard;
     const Tensor xr = rows(x), gr = rows(gate);
+    // what the checks above cannot tell: rows with gaps between them
+    TORCH_CHECK(!rows_meet(xr, state) && !rows_meet(gr, state),
+                "x and gate must not share memory with state, which is written in place");
     const Tensor sl = slots.defined() ? slots.contiguous() : Tensor();
     out = at::empty(x.sizes(), x.options());
     check_rc(ltc_gated_scan_step(ptr(xr), xr.stride(0), ptr(gr), gr.stride(0), fp(state),
