@@ -408,8 +408,10 @@ class _HipModule:
             if tuple(t.shape) != tuple(shp):
                 raise ValueError(f"tensor shape {tuple(t.shape)} != expected {tuple(shp)}")
 
-    def ltc_sensory_fwd(self, inputs, sensory_sigma, sensory_mu, sensory_w_pos, sensory_erev):
-        """One step's sensory sums -> [w_num_sensory (B,H), w_den_sensory (B,H)]."""
+    def ltc_sensory_fwd(self, inputs, sensory_sigma, sensory_mu, sensory_w_pos, sensory_erev,
+                        *, out=None):
+        """One step's sensory sums -> [w_num_sensory (B,H), w_den_sensory (B,H)], in
+        contiguous float32 tensors of the caller's if `out` holds two."""
         if inputs.dim() != 2:
             raise ValueError(f"inputs must be (B, D), got {tuple(inputs.shape)}")
         B, D = inputs.shape
@@ -420,7 +422,7 @@ class _HipModule:
         self._check_f32(dev, inputs, *params)
         params = [p.contiguous() for p in params]
         f32 = dict(device=dev, dtype=torch.float32)
-        wn, wd = torch.empty(B, H, **f32), torch.empty(B, H, **f32)
+        wn, wd = out if out is not None else (torch.empty(B, H, **f32), torch.empty(B, H, **f32))
         need = self.capi.sizes("sfwd_ws", B, 1, D, H, 1)
         with torch.cuda.device(dev):
             ws = _workspace(need, dev)
@@ -459,8 +461,9 @@ class _HipModule:
         return [out, vbuf]
 
     def ltc_sensory_bwd(self, grad_w_num, grad_w_den, inputs, sensory_sigma, sensory_mu,
-                        sensory_w_pos, sensory_erev):
-        """-> [grad_inputs (B,D), grad_sigma, grad_mu, grad_w_pos, grad_erev (D,H)]."""
+                        sensory_w_pos, sensory_erev, *, grad_inputs=None):
+        """-> [grad_inputs (B,D), grad_sigma, grad_mu, grad_w_pos, grad_erev (D,H)], the
+        first in a contiguous float32 tensor of the caller's if given."""
         if inputs.dim() != 2:
             raise ValueError(f"inputs must be (B, D), got {tuple(inputs.shape)}")
         B, D = inputs.shape
@@ -473,7 +476,8 @@ class _HipModule:
         params = [p.contiguous() for p in params]
         gn, gd = grad_w_num.contiguous(), grad_w_den.contiguous()
         f32 = dict(device=dev, dtype=torch.float32)
-        grads = [torch.empty(B, D, **f32)] + [torch.empty(D, H, **f32) for _ in range(4)]
+        gx = grad_inputs if grad_inputs is not None else torch.empty(B, D, **f32)
+        grads = [gx] + [torch.empty(D, H, **f32) for _ in range(4)]
         need = self.capi.sizes("sbwd_ws", B, 1, D, H, 1)
         with torch.cuda.device(dev):
             ws = _workspace(need, dev)
@@ -862,20 +866,61 @@ def ltc_cuda_forward(x_seq, state, w_pos, w_erev, mu, sigma,
         cm_t, gleak_pos, vleak, ode_unfolds, epsilon, needs_grad)
 
 
+# Workspace that may grow with the rows of one call of the sensory entry points.
+SENSORY_ROW_BYTES = 1 << 32
+
+
+def _sensory_blocks(N, D, H, backward):
+    """Cuts N rows into blocks of about one size, [(first, end), ...].
+
+    The entry points are made for one time step's batch. For each row their workspace
+    holds the padded sums, and in the backward dL/dx of every 32 neurons apart, which
+    for 32768 rows of 2048 inputs and neurons is 18 GB where dL/dx itself is 0.27. Every
+    block forms the synapses' images again and sums its own parameter gradients: those
+    rows' backward takes 55.6 ms in one, 56.1 in blocks of 4 GiB, 58.9 in blocks of 1.
+    So 4 GiB, and 1024 rows at least, where rows are very wide. At most 2^20: the
+    forward's grid holds 65535 blocks of 32.
+    """
+    Hp, Dp = -(-H // 64) * 64, -(-D // 64) * 64
+    row = 4 * (2 * Hp + (Hp // 32 * Dp if backward else 0))
+    most = min(max(SENSORY_ROW_BYTES // row, 1024), 1 << 20)
+    n = max(1, -(-N // most))
+    per = -(-N // n)
+    return [(i * per, min(N, (i + 1) * per)) for i in range(n)]
+
+
 class LTCSensoryFunction(torch.autograd.Function):
     """The sensory sums of every row, [w_num, w_den] (N, H), with their gradients: the
-    per-step entry points ltc_sensory_fwd / ltc_sensory_bwd over all rows at once."""
+    per-step entry points ltc_sensory_fwd / ltc_sensory_bwd over blocks of rows, all at
+    once where they are few. The blocks' parameter gradients are added in order."""
 
     @staticmethod
     def forward(ctx, inputs, sigma, mu, w_pos, erev):
         ctx.save_for_backward(inputs, sigma, mu, w_pos, erev)
-        return tuple(require_kernels().ltc_sensory_fwd(inputs, sigma, mu, w_pos, erev))
+        k, (N, D), H = require_kernels(), inputs.shape, sigma.shape[-1]
+        blocks = _sensory_blocks(N, D, H, False)
+        if len(blocks) == 1:
+            return tuple(k.ltc_sensory_fwd(inputs, sigma, mu, w_pos, erev))
+        num, den = (torch.empty(N, H, device=inputs.device, dtype=torch.float32) for _ in range(2))
+        for i, j in blocks:
+            k.ltc_sensory_fwd(inputs[i:j], sigma, mu, w_pos, erev, out=(num[i:j], den[i:j]))
+        return num, den
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_num, g_den):
-        g = require_kernels().ltc_sensory_bwd(g_num, g_den, *ctx.saved_tensors)
-        return tuple(g)
+        inputs, *params = ctx.saved_tensors
+        k, (N, D) = require_kernels(), inputs.shape
+        blocks = _sensory_blocks(N, D, params[0].shape[-1], True)
+        if len(blocks) == 1:
+            return tuple(k.ltc_sensory_bwd(g_num, g_den, inputs, *params))
+        gx = torch.empty(N, D, device=inputs.device, dtype=torch.float32)
+        total = None
+        for i, j in blocks:
+            g = k.ltc_sensory_bwd(g_num[i:j], g_den[i:j], inputs[i:j], *params,
+                                  grad_inputs=gx[i:j])[1:]
+            total = g if total is None else [a.add_(b) for a, b in zip(total, g)]
+        return (gx, *total)
 
 
 def ltc_sensory_sums(inputs, sigma, mu, w_pos, erev):
