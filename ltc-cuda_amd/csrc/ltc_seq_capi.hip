@@ -126,9 +126,12 @@ int check_top(int V, int top) {
   return LTC_OK;
 }
 
+// log2(e) / t, by which the kernels scale: they would take 0 times an infinity.
+float logit_scale(float t) { return (float)(1.4426950408889634 / (double)t); }
+
 int check_temperature(float t) {
-  if (!(t > 0.f) || !(t < __builtin_inff()) || !(1.f / t < __builtin_inff()))
-    return host_fail(LTC_EINVAL, "temperature must be positive and finite");
+  if (!(t > 0.f) || !(t < __builtin_inff()) || !(logit_scale(t) < __builtin_inff()))
+    return host_fail(LTC_EINVAL, "temperature must be positive and finite, and so must log2(e) over it");
   return LTC_OK;
 }
 
@@ -144,7 +147,7 @@ ltc::TokArgs tok_args(const void* x, long long sx, const void* ids, int id64, in
   a.V = V;
   a.tau = temperature;
   a.inv_tau = 1.f / temperature;
-  a.c = (float)(1.4426950408889634 / (double)temperature);
+  a.c = logit_scale(temperature);
   a.top = top;
   ltc::tok_split(N, V, type_bytes(type), top, &a.nsplit, &a.seg);
   return a;
