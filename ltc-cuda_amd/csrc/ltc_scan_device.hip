@@ -32,7 +32,11 @@ constexpr int kMarkNone = -1, kMarkStart = 1, kMarkEnd = 2;
 // a and 1 - a (decay: 1), each to its own relative precision: with e = exp(-g),
 // a = 1 / (1 + e) and 1 - a = e a. e is kept below 2^126, where a is 2^-126 and
 // 1 - a is 1; `minimum` passes a NaN on.
-// exp_of is e, or in the other form a itself, from which gate_from goes on.
+// exp_of is e, or in the other form a itself, from which gate_from goes on. g log2(e) is
+// one rounded product, which leaves exp2 of it off by |g| 2^-24 relative. That is more
+// than an ulp only where |g| is over 1: there a, or 1 - a, is small and carries the error,
+// which the other side takes on times the same smallness. A product in two parts would
+// cost an instruction a gate in kernels that are bound by theirs.
 template <int FORM>
 __device__ __forceinline__ float exp_of(float g) {
   return FORM == LTC_GATE_BLEND

@@ -372,8 +372,11 @@ def _gated_scan_plain(x, gate, state, cu_seqlens=None):
 
 
 class _ScaleColumns(torch.autograd.Function):
-    """w (D, H) times s (H,). The gradient of s is summed by halves: torch's own
-    reduction over many rows is replayed wrongly in a captured graph."""
+    """w (D, H) times s (H,). The gradient of s is summed by halves. torch's reduction
+    over many rows takes several workgroups, whose counters a memset node clears in a
+    captured graph, and on ROCm 7.2 such graphs give other sums from the second replay
+    on (torch 2.10: the gradient of a Linear(32, 700)'s bias over 600 rows, while one
+    reduction alone in a graph is right)."""
 
     @staticmethod
     def forward(ctx, w, s):
@@ -407,6 +410,9 @@ class LinearTimeConstant(nn.Module):
     float32, as that layer. forward also takes packed sequences: x_seq (tokens, D)
     with cu_seqlens (int32, sequences + 1). step() advances streams by one token for
     serving, their states updated in place, in rows of a pool if slots are given.
+
+    The gate goes by a logarithm here and an exponential in the scan, each to a few
+    roundings, since the scan takes pre-activations.
     """
 
     def __init__(
@@ -517,7 +523,8 @@ class TokenReadout(nn.Module):
     distill(h, teacher_logits, teacher_ids) -> ltc_cuda.ltc_top_distill's loss of each
     row. The logits are in the readout's own type (float32, bfloat16 or float16), what
     is made of them in float32. There is no bias: torch forms its gradient with a
-    reduction that a captured graph replays wrongly. CPU tensors take plain torch.
+    reduction that a captured graph replays wrongly (_ScaleColumns). CPU tensors take
+    plain torch, which raises for an id past the vocabulary where the kernels give NaN.
     """
 
     def __init__(self, hidden_dim: int, vocab: int, dtype=None):

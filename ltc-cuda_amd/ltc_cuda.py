@@ -994,7 +994,8 @@ def ltc_token_logprobs(logits, ids, top=0, temperature=1.0):
     tokens, equal logits by the lower id. All but the ids are float32. Rows with a
     negative id have no token: 0 and 0, and no gradient; an id of V or more gives
     NaN. Logits of -inf have probability 0. Gradients reach logits through logp and
-    entropy; the alternatives carry none.
+    entropy; the alternatives carry none. Rows of one stride are read where they are;
+    others (logits[:, :-1] of a batch) are copied, in the forward and in the backward.
     """
     return tuple(_require_ext().token_logprobs(logits, ids, int(top), float(temperature)))
 
@@ -1006,7 +1007,8 @@ def ltc_top_distill(logits, teacher_logits, teacher_ids, temperature=1.0):
     teacher_logits (..., K) / temperature over the entries that are there (a
     negative id is one that is not) and q = softmax(logits (..., V) / temperature).
     K <= 1024. A row without entries gives 0 and no gradient; an id of V or more
-    gives NaN. Gradients reach logits only; the teacher's have to be detached.
+    gives NaN. Gradients reach logits only; the teacher's have to be detached. Logits
+    are read in place or copied as ltc_token_logprobs' are.
     """
     return _require_ext().top_distill(logits, teacher_logits, teacher_ids, float(temperature))
 
