@@ -2,12 +2,9 @@
 #pragma once
 
 #include <torch/extension.h>
-#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <c10/core/impl/TorchDispatchModeTLS.h>
-
-#include <initializer_list>
 
 namespace ltc_torch {
 
@@ -17,7 +14,7 @@ namespace ltc_torch {
 // a word. So both are errors.
 inline void check_modes(const char* name, at::ArrayRef<torch::Tensor> inputs) {
   for (const torch::Tensor& t : inputs)
-    TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(t), name,
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), name,
                                 " has no forward-mode derivative");
   TORCH_CHECK_NOT_IMPLEMENTED(
       !torch::jit::tracer::isTracing() &&
