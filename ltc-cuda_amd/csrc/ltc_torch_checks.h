@@ -12,10 +12,14 @@ namespace ltc_torch {
 // forward-mode differentiation nor a tracer looks: the one would take the tangent
 // for zero, the other would record the outputs' allocation alone, and both without
 // a word. So both are errors.
-inline void check_modes(const char* name, at::ArrayRef<torch::Tensor> inputs) {
-  for (const torch::Tensor& t : inputs)
-    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), name,
-                                " has no forward-mode derivative");
+inline void check_tangent(const char* name, const torch::Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), name,
+                              " has no forward-mode derivative");
+}
+
+template <class... Tensors>
+void check_modes(const char* name, const Tensors&... inputs) {
+  (check_tangent(name, inputs), ...);
   TORCH_CHECK_NOT_IMPLEMENTED(
       !torch::jit::tracer::isTracing() &&
           !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY),

@@ -168,8 +168,8 @@ std::vector<Tensor> module_apply(const Tensor& x, const c10::optional<Tensor>& s
                                  const std::vector<Tensor>& leaves, double dt, int64_t U,
                                  double eps, double ln_eps) {
   const Tensor state = state_opt.has_value() ? *state_opt : Tensor();
-  ltc_torch::check_modes("ltc_module_forward", {x, state});
-  ltc_torch::check_modes("ltc_module_forward", leaves);
+  ltc_torch::check_modes("ltc_module_forward", x, state);
+  for (const Tensor& t : leaves) ltc_torch::check_tangent("ltc_module_forward", t);
   check_inputs(x, state, leaves);
   const bool needs_grad = torch::GradMode::is_enabled() &&
                           torch::autograd::compute_requires_grad(x, state, leaves);

@@ -220,7 +220,7 @@ struct GatedScanBackward : public Node {
 std::vector<Tensor> gated_scan(const Tensor& x, const Tensor& gate, const OptTensor& state_opt,
                                const OptTensor& cu_opt, int64_t form) {
   const Tensor state = state_opt.value_or(Tensor()), cu = cu_opt.value_or(Tensor());
-  check_modes("ltc_gated_scan", {x, gate, state});
+  check_modes("ltc_gated_scan", x, gate, state);
   const ScanShape s = check_scan(x, gate, state, cu);
   check_device(x, x, "x");
   const bool needs_grad =
@@ -288,7 +288,7 @@ bool rows_meet(const Tensor& t, const Tensor& table) {
 
 Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& state, const OptTensor& slots_opt,
                        int64_t form) {
-  check_modes("ltc_gated_scan_step", {x, gate, state});
+  check_modes("ltc_gated_scan_step", x, gate, state);
   TORCH_CHECK_VALUE(x.dim() == 2, "x must be (B, H), got ", x.sizes());
   type_of(x, "x");
   TORCH_CHECK_TYPE(gate.scalar_type() == x.scalar_type() || gate.scalar_type() == at::kFloat,
@@ -406,7 +406,7 @@ struct TokenLogprobsBackward : public Node {
 
 std::vector<Tensor> token_logprobs(const Tensor& logits, const Tensor& ids, int64_t top,
                                    double temperature) {
-  check_modes("ltc_token_logprobs", {logits});
+  check_modes("ltc_token_logprobs", logits);
   const Rows r = check_logits(logits);
   const int id64 = check_ids(ids, logits, "ids");
   const auto shape = logits.sizes().slice(0, logits.dim() - 1);
@@ -486,7 +486,7 @@ struct TopDistillBackward : public Node {
 };
 
 Tensor top_distill(const Tensor& logits, const Tensor& teacher, const Tensor& ids, double temperature) {
-  check_modes("ltc_top_distill", {logits, teacher});
+  check_modes("ltc_top_distill", logits, teacher);
   const Rows r = check_logits(logits);
   const int id64 = check_ids(ids, logits, "teacher_ids");
   type_of(teacher, "teacher_logits");
