@@ -342,7 +342,8 @@ int ltc_gated_scan_step(const void* x, long long sxb, const void* gate, long lon
   host_clear_error();
   int rc = check_scan_call(x, gate, nullptr, x_type, gate_type, form, B, 1, H);
   if (rc != LTC_OK) return rc;
-  if (P < 0 || (!slots && P != B))
+  // slots of no rows have no address
+  if (P < 0 || (!slots && B > 0 && P != B))
     return host_fail(LTC_EINVAL, "P must be the states' number, B without slots");
   // rows are the grid's second dimension
   if (B > 65535) return host_fail(LTC_EUNSUPPORTED, "more than 65535 rows in a step");
