@@ -382,6 +382,7 @@ int ltc_gated_scan_step(const void* x, long long sxb, const void* gate, long lon
  *   top_logp, top_ids   (N,top) fp32 and int64, most probable first, equal logits by
  *                the lower id; every row, with a token or not. top <= LTC_TOP_MAX
  *                and <= V; 0 for none
+ *   temperature  positive and finite, as log2(e) over it is (4.3e-39 and up)
  *   stats        (N,3) fp32 for the backward, or NULL
  * A logit of -inf has probability 0; a row of nothing else, or with a NaN or +inf,
  * gives NaN (in such a row top_ids are in range, but otherwise unspecified).
