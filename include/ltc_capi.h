@@ -24,7 +24,8 @@
  *    launched), LTC_EUNSUPPORTED for shapes outside the supported range,
  *    LTC_EHIP when a HIP call or launch fails. ltc_last_error() then holds a
  *    message (thread-local).
- *  - Results are deterministic: no atomics; every reduction has a fixed order.
+ *  - Results are deterministic: every reduction of floating-point numbers has a fixed
+ *    order (atomics count whole numbers only).
  */
 #ifndef LTC_CAPI_H
 #define LTC_CAPI_H
@@ -428,6 +429,166 @@ int ltc_top_distill_backward(const void* logits, long long sl, const void* teach
                              int logits_type, int teacher_type, long long N, int V, int K,
                              float temperature, const float* stats, const float* grad_loss,
                              long long sgl, void* grad_logits, void* stream);
+
+/*
+ * Operators of a token model around the layer: what brings tokens in, mixes them and
+ * adjusts the scores of the next. No counterpart in the reference. Types, workspaces and
+ * determinism as above.
+ */
+
+/* Activations: none; v / (1 + exp(-v)). */
+#define LTC_ACT_NONE 0
+#define LTC_ACT_SILU 1
+
+/*
+ * Short causal convolution of each channel, over B sequences of T steps or packed ones
+ * (cu_seqlens as in ltc_gated_scan_forward):
+ *   out_t = act(bias + sum_k weight[:,k] in_{t-K+1+k}),
+ * where in is the sequence with its state, its last K-1 inputs, before it.
+ *   x            (B,T,C) with element strides sxb, sxt; packed (T,C), stride sxt
+ *   weight       (C,K) contiguous; its type is x's or LTC_F32. K <= LTC_CONV_TAPS_MAX
+ *   bias         (C), weight's type, or NULL for none
+ *   state        (B,K-1,C) contiguous, x's type, or NULL for zero
+ *   out          (B,T,C) or (T,C), contiguous, x's type
+ *   state_final  (B,K-1,C) contiguous: the last K-1 inputs, the state's own among them
+ *                where a sequence is shorter
+ * The backward takes grad_out (NULL for zero; strides sob, sot) and grad_state_final
+ * (contiguous, or NULL for zero). Its outputs are contiguous, of their input's type, and
+ * each may be NULL where it is not wanted.
+ */
+#define LTC_CONV_TAPS_MAX 8
+long long ltc_causal_conv_bwd_workspace_bytes(int x_type, int B, int T, int C, int K, int packed);
+int ltc_causal_conv_forward(const void* x, long long sxb, long long sxt, const void* weight,
+                            const void* bias, const void* state, const int* cu_seqlens,
+                            int x_type, int weight_type, int activation, int B, int T, int C,
+                            int K, void* out, void* state_final, void* stream);
+int ltc_causal_conv_backward(const void* x, long long sxb, long long sxt, const void* weight,
+                             const void* bias, const void* state, const int* cu_seqlens,
+                             int x_type, int weight_type, int activation, int B, int T, int C,
+                             int K, const void* grad_out, long long sob, long long sot,
+                             const void* grad_state_final, void* grad_x, void* grad_weight,
+                             void* grad_bias, void* grad_state, void* workspace,
+                             long long workspace_bytes, void* stream);
+
+/*
+ * One token of B streams: out[b], and x[b] joins the stream's last inputs, the oldest
+ * leaving. state (P,K-1,C) with strides ssp, sst and 1, its rows apart; slots as in
+ * ltc_gated_scan_step.
+ */
+int ltc_causal_conv_step(const void* x, long long sxb, const void* weight, const void* bias,
+                         void* state, long long ssp, long long sst, const int* slots,
+                         int x_type, int weight_type, int activation, int B, int C, int K,
+                         int P, void* out, void* stream);
+
+/*
+ * Selective state space scan, over B sequences of T steps or packed ones. Of channel h in
+ * group g = h / (H / G), and state n:
+ *   s_t = delta_t + delta_bias, or softplus of it
+ *   v_t = exp(s_t A[h,n]) v_{t-1} + s_t B_t[g,n] x_t
+ *   out_t = (sum_n C_t[g,n] v_t + D x_t) silu(z_t)      (without z: no factor)
+ *   x, delta, z  (B,T,H) with element strides s.b, s.t; packed (T,H), stride s.t; z NULL
+ *                for none
+ *   A            (H,N) fp32 contiguous; taken as it is: above 0 states may grow without
+ *                bound. N <= LTC_STATES_MAX
+ *   B, C         (B,T,G,N) with element strides s.b, s.t, s.g; packed (T,G,N)
+ *   D, delta_bias   (H) fp32, or NULL for none
+ *   state        (B,H,N) fp32 contiguous, or NULL for zero
+ *   out          (B,T,H) or (T,H), contiguous
+ *   state_final  (B,H,N) fp32 contiguous: the last state; an empty sequence's initial one
+ *   saved        ltc_selective_scan_saved_floats() floats, written when save is nonzero,
+ *                for the backward of the same inputs
+ * x, delta, z, B, C, out and their gradients have one type. Tokens outside every sequence
+ * give zeros, in out and in the gradients, whatever lies there.
+ */
+#define LTC_STATES_MAX 64
+long long ltc_selective_scan_saved_floats(int B, int T, int H, int N, int G, int packed);
+long long ltc_selective_scan_fwd_workspace_bytes(int B, int T, int H, int N, int G, int packed);
+long long ltc_selective_scan_bwd_workspace_bytes(int B, int T, int H, int N, int G, int packed);
+int ltc_selective_scan_forward(const void* x, long long sxb, long long sxt, const void* delta,
+                               long long sdb, long long sdt, const float* A, const void* Bm,
+                               long long sbb, long long sbt, long long sbg, const void* Cm,
+                               long long scb, long long sct, long long scg, const float* D,
+                               const void* z, long long szb, long long szt,
+                               const float* delta_bias, const float* state,
+                               const int* cu_seqlens, int type, int delta_softplus, int B,
+                               int T, int H, int N, int G, int save, void* out,
+                               float* state_final, float* saved, void* workspace,
+                               long long workspace_bytes, void* stream);
+/* grad_out (NULL for zero) has strides sob, sot; grad_state_final is contiguous or NULL for
+ * zero. The gradients are contiguous, of their input's shape and type; each may be NULL
+ * where it is not wanted. */
+int ltc_selective_scan_backward(const void* x, long long sxb, long long sxt, const void* delta,
+                                long long sdb, long long sdt, const float* A, const void* Bm,
+                                long long sbb, long long sbt, long long sbg, const void* Cm,
+                                long long scb, long long sct, long long scg, const float* D,
+                                const void* z, long long szb, long long szt,
+                                const float* delta_bias, const float* state,
+                                const int* cu_seqlens, int type, int delta_softplus, int B,
+                                int T, int H, int N, int G, const float* saved,
+                                const void* grad_out, long long sob, long long sot,
+                                const float* grad_state_final, void* grad_x, void* grad_delta,
+                                float* grad_A, void* grad_B, void* grad_C, float* grad_D,
+                                void* grad_z, float* grad_delta_bias, float* grad_state,
+                                void* workspace, long long workspace_bytes, void* stream);
+
+/*
+ * One token of B streams: x, delta, z (B,H) with row strides, B and C (B,G,N); state
+ * (P,H,N) fp32, row stride ssp (at least H N), written over; slots as in
+ * ltc_gated_scan_step.
+ */
+int ltc_selective_scan_step(const void* x, long long sx, const void* delta, long long sd,
+                            const float* A, const void* Bm, long long sbb, long long sbg,
+                            const void* Cm, long long scb, long long scg, const float* D,
+                            const void* z, long long sz, const float* delta_bias, float* state,
+                            long long ssp, const int* slots, int type, int delta_softplus,
+                            int B, int H, int N, int G, int P, void* out, void* stream);
+
+/*
+ * Embedding: out[i] = scale table[ids[i]].
+ *   table        (V,H), row stride st
+ *   ids          (n) int32 or (ids64 nonzero) int64. A negative id is a token that is not
+ *                there: a row of zeros and no gradient; one of V or more gives NaN and
+ *                no gradient
+ *   out          (n,H) contiguous, the table's type
+ * The backward writes grad_table (V,H) contiguous, every row: scale times the sum of
+ * grad_out (n,H; row stride so) over the row's tokens, in their order.
+ */
+int ltc_embed_forward(const void* table, long long st, const void* ids, int ids64, int type,
+                      long long n, int V, int H, float scale, void* out, void* stream);
+long long ltc_embed_bwd_workspace_bytes(long long n, int V, int H);
+int ltc_embed_backward(const void* ids, int ids64, int type, long long n, int V, int H,
+                       float scale, const void* grad_out, long long so, void* grad_table,
+                       void* workspace, long long workspace_bytes, void* stream);
+
+/*
+ * Logits adjusted for the choice of the next token. In fp32, of token v in row r, x its
+ * logit, and in this order:
+ *   v occurs in the context:               x / repetition where x > 0, else x repetition
+ *   v occurs c > 0 times after the prompt: x - frequency c - presence
+ *   v is in the list of biases:            plus the sum of its biases, in their order
+ *   v is not allowed by the mask:          -inf, whatever x is
+ *   logits       (R,V), row stride sl
+ *   context      (R,ctx) int32 or (context64 nonzero) int64, row stride sc. Entries
+ *                outside 0 ... V-1 are not there. ctx 0 for none
+ *   prompt_lens  (R) int32: the entries of the context that are the prompt, its first; NULL
+ *                for 0
+ *   repetition, frequency, presence   (R) fp32, or NULL for the values of the same name
+ *                with a 0, which are finite, repetition0 positive
+ *   bias_ids     (R,K) int32 or int64, row stride sbi, entries outside 0 ... V-1 not there;
+ *                bias (R,K) fp32, row stride sb. K <= LTC_BIAS_MAX, 0 for none
+ *   mask         (R, (V + 31) / 32) int32 words, row stride sm: token v is allowed where
+ *                bit v % 32 of word v / 32 is set; NULL for all
+ *   out          (R,V) contiguous, the logits' type
+ * Row strides of 0 share a row among all.
+ */
+#define LTC_BIAS_MAX 1024
+int ltc_adjust_logits(const void* logits, long long sl, const void* context, long long sc,
+                      int context64, int ctx, const int* prompt_lens, const float* repetition,
+                      const float* frequency, const float* presence, float repetition0,
+                      float frequency0, float presence0, const void* bias_ids, long long sbi,
+                      int bias_ids64, const float* bias, long long sb, int K, const int* mask,
+                      long long sm, int logits_type, long long R, int V, void* out,
+                      void* stream);
 
 /*
  * Launch plan of one call, for diagnostics and host-side bounds tests. No

@@ -19,7 +19,10 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_NAME = "libltc_hip.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 SOURCES = ("ltc_device.hip", "ltc_capi.hip", "ltc_scan_device.hip", "ltc_token_device.hip",
-           "ltc_seq_capi.hip")
+           "ltc_seq_capi.hip", "ltc_conv_device.hip", "ltc_ssm_device.hip",
+           "ltc_vocab_device.hip", "ltc_model_capi.hip")
+HEADERS = ("ltc_internal.h", "ltc_seq_internal.h", "ltc_model_internal.h", "ltc_capi_util.h",
+           "ltc_vec.h", "ltc_tokens.h", "ltc_torch_checks.h", "ltc_torch_util.h")
 ARCH = os.environ.get("LTC_OFFLOAD_ARCH", "gfx950")
 
 
@@ -34,9 +37,7 @@ def source_files() -> list:
     """Every file the library and the torch extension are built from."""
     inc = os.path.join(os.path.dirname(HERE), "include", "ltc_capi.h")
     return [os.path.join(CSRC, s) for s in SOURCES] + [
-        os.path.join(CSRC, "ltc_internal.h"), os.path.join(CSRC, "ltc_seq_internal.h"),
-        os.path.join(CSRC, "ltc_vec.h"), os.path.join(CSRC, "ltc_torch_checks.h"),
-        *[os.path.join(CSRC, s) for s in EXT_SOURCES], inc]
+        *[os.path.join(CSRC, s) for s in HEADERS + EXT_SOURCES], inc]
 
 
 def command(out: str = LIB_PATH, arch: str = ARCH) -> list:
@@ -61,7 +62,7 @@ def command(out: str = LIB_PATH, arch: str = ARCH) -> list:
     ]
 
 
-EXT_SOURCES = ("ltc_torch_ext.cpp", "ltc_torch_seq.cpp")
+EXT_SOURCES = ("ltc_torch_ext.cpp", "ltc_torch_seq.cpp", "ltc_torch_model.cpp")
 EXT_NAME = "_ltc_torch"
 
 
@@ -72,7 +73,7 @@ def ext_path() -> str:
 
 def ext_command(out: str) -> list:
     """Host-only C++ build of the torch glue (the autograd nodes of the fused
-    module path and of the sequence and token operators), linked against libltc_hip.so through $ORIGIN."""
+    module path and of the sequence, token and model operators), linked against libltc_hip.so through $ORIGIN."""
     import sysconfig
     import torch
     from torch.utils import cpp_extension as ce

@@ -713,7 +713,10 @@ const char* const kNames[ltc::K_COUNT] = {"ltc_prep",     "ltc_sens_fwd", "ltc_o
                                           "ltc_ln_bwd",   "ltc_finalize",
                                           "ltc_scan_fwd", "ltc_scan_bwd", "ltc_scan_step",
                                           "ltc_logprobs_fwd", "ltc_logprobs_bwd",
-                                          "ltc_distill_fwd", "ltc_distill_bwd"};
+                                          "ltc_distill_fwd", "ltc_distill_bwd",
+                                          "ltc_conv_fwd", "ltc_conv_bwd", "ltc_conv_step",
+                                          "ltc_ssm_fwd",  "ltc_ssm_bwd",  "ltc_ssm_step",
+                                          "ltc_embed_fwd", "ltc_embed_bwd", "ltc_adjust"};
 
 struct Timing {
   std::mutex mu;

@@ -66,6 +66,15 @@ enum KernelId : int {
   K_LOGPROBS_BWD,
   K_DISTILL_FWD,
   K_DISTILL_BWD,
+  K_CONV_FWD,
+  K_CONV_BWD,
+  K_CONV_STEP,
+  K_SSM_FWD,
+  K_SSM_BWD,
+  K_SSM_STEP,
+  K_EMBED_FWD,
+  K_EMBED_BWD,
+  K_ADJUST,
   K_COUNT
 };
 

@@ -76,6 +76,12 @@ class CApi:
         "ltc_token_logprobs_workspace_bytes", "ltc_token_logprobs_forward",
         "ltc_token_logprobs_backward", "ltc_top_distill_workspace_bytes",
         "ltc_top_distill_forward", "ltc_top_distill_backward",
+        "ltc_causal_conv_bwd_workspace_bytes", "ltc_causal_conv_forward",
+        "ltc_causal_conv_backward", "ltc_causal_conv_step", "ltc_selective_scan_saved_floats",
+        "ltc_selective_scan_fwd_workspace_bytes", "ltc_selective_scan_bwd_workspace_bytes",
+        "ltc_selective_scan_forward", "ltc_selective_scan_backward", "ltc_selective_scan_step",
+        "ltc_embed_forward", "ltc_embed_bwd_workspace_bytes", "ltc_embed_backward",
+        "ltc_adjust_logits",
     )
     PLAN_FIELDS = ("Hp", "Dp", "NB", "KS", "RC", "threads", "lds_fwd", "lds_bwd", "NCH",
                    "NRC", "ode_workgroups", "fuse", "KSB", "RCB",
@@ -192,6 +198,49 @@ class CApi:
         lib.ltc_top_distill_backward.restype = _int
         lib.ltc_top_distill_backward.argtypes = (
             _dist + [_f32p, _f32p, _i64, _f32p, ctypes.c_void_p])
+        lib.ltc_causal_conv_bwd_workspace_bytes.restype = _i64
+        lib.ltc_causal_conv_bwd_workspace_bytes.argtypes = [_int] * 6
+        _conv = [_f32p, _i64, _i64] + [_f32p] * 4 + [_int] * 7
+        lib.ltc_causal_conv_forward.restype = _int
+        lib.ltc_causal_conv_forward.argtypes = _conv + [_f32p, _f32p, ctypes.c_void_p]
+        lib.ltc_causal_conv_backward.restype = _int
+        lib.ltc_causal_conv_backward.argtypes = (
+            _conv + [_f32p, _i64, _i64] + [_f32p] * 6 + [_i64, ctypes.c_void_p])
+        lib.ltc_causal_conv_step.restype = _int
+        lib.ltc_causal_conv_step.argtypes = (
+            [_f32p, _i64, _f32p, _f32p, _f32p, _i64, _i64, _f32p] + [_int] * 7
+            + [_f32p, ctypes.c_void_p])
+        for name in ("ltc_selective_scan_saved_floats", "ltc_selective_scan_fwd_workspace_bytes",
+                     "ltc_selective_scan_bwd_workspace_bytes"):
+            fn = getattr(lib, name)
+            fn.restype = _i64
+            fn.argtypes = [_int] * 6
+        _ssm = ([_f32p, _i64, _i64] * 2 + [_f32p] + [_f32p, _i64, _i64, _i64] * 2
+                + [_f32p, _f32p, _i64, _i64, _f32p, _f32p, _f32p] + [_int] * 7)
+        lib.ltc_selective_scan_forward.restype = _int
+        lib.ltc_selective_scan_forward.argtypes = (
+            _ssm + [_int] + [_f32p] * 4 + [_i64, ctypes.c_void_p])
+        lib.ltc_selective_scan_backward.restype = _int
+        lib.ltc_selective_scan_backward.argtypes = (
+            _ssm + [_f32p, _f32p, _i64, _i64] + [_f32p] * 11 + [_i64, ctypes.c_void_p])
+        lib.ltc_selective_scan_step.restype = _int
+        lib.ltc_selective_scan_step.argtypes = (
+            [_f32p, _i64] * 2 + [_f32p] + [_f32p, _i64, _i64] * 2
+            + [_f32p, _f32p, _i64, _f32p, _f32p, _i64, _f32p] + [_int] * 7
+            + [_f32p, ctypes.c_void_p])
+        lib.ltc_embed_forward.restype = _int
+        lib.ltc_embed_forward.argtypes = [_f32p, _i64, _f32p, _int, _int, _i64, _int, _int, _flt,
+                                          _f32p, ctypes.c_void_p]
+        lib.ltc_embed_bwd_workspace_bytes.restype = _i64
+        lib.ltc_embed_bwd_workspace_bytes.argtypes = [_i64, _int, _int]
+        lib.ltc_embed_backward.restype = _int
+        lib.ltc_embed_backward.argtypes = [_f32p, _int, _int, _i64, _int, _int, _flt, _f32p, _i64,
+                                           _f32p, _f32p, _i64, ctypes.c_void_p]
+        lib.ltc_adjust_logits.restype = _int
+        lib.ltc_adjust_logits.argtypes = (
+            [_f32p, _i64, _f32p, _i64, _int, _int] + [_f32p] * 4 + [_flt] * 3
+            + [_f32p, _i64, _int, _f32p, _i64, _int, _f32p, _i64, _int, _i64, _int, _f32p,
+               ctypes.c_void_p])
         lib.ltc_scan_status.restype = _int
         lib.ltc_scan_status.argtypes = [_int]
         lib.ltc_device_status.restype = _int
@@ -1011,6 +1060,125 @@ def ltc_top_distill(logits, teacher_logits, teacher_ids, temperature=1.0):
     are read in place or copied as ltc_token_logprobs' are.
     """
     return _require_ext().top_distill(logits, teacher_logits, teacher_ids, float(temperature))
+
+
+# ---------------------------------------------------- operators of a token model
+
+# ltc_causal_conv's activations, as include/ltc_capi.h numbers them.
+ACTIVATIONS = {None: 0, "silu": 1}
+
+
+def _activation(name) -> int:
+    if name not in ACTIVATIONS:
+        raise ValueError(f"activation must be None or 'silu', got {name!r}")
+    return ACTIVATIONS[name]
+
+
+def ltc_causal_conv(x, weight, bias=None, state=None, cu_seqlens=None, activation=None):
+    """Short causal convolution of each channel -> (out, state_final).
+
+    out_t = act(bias + sum_k weight[:, k] in_{t-K+1+k}), with in the sequence and its
+    state, the K-1 inputs before it, in front.
+
+    x       (B, T, C), float32, bfloat16 or float16; with cu_seqlens (tokens, C)
+    weight  (C, K), K from 1 to 8; x's type or float32
+    bias    (C,), weight's type, or None
+    state   (B, K-1, C), x's type, oldest first, or None for zero
+    cu_seqlens  as in ltc_gated_scan
+    activation  None, or "silu": v / (1 + exp(-v))
+    out     x's shape and type; state_final as state: the last K-1 inputs, the state's
+            own among them where a sequence is shorter.
+
+    Sums are float32. Gradients reach x, weight, bias and state through both outputs.
+    """
+    return tuple(_require_ext().causal_conv(x, weight, bias, state, cu_seqlens,
+                                            _activation(activation)))
+
+
+def ltc_causal_conv_step(x, weight, state, bias=None, slots=None, activation=None):
+    """One token of each stream: returns out (B, C) and updates `state` in place.
+
+    x (B, C); state (B, K-1, C), or with slots (int32 (B,)) a pool (P, K-1, C) whose row
+    slots[b] is row b's. Slots as in ltc_gated_scan_step: a negative one is padding, one
+    of P or more gives NaN, and rows that name one slot are taken in their order. No
+    backward.
+    """
+    return _require_ext().causal_conv_step(x, weight, state, bias, slots, _activation(activation))
+
+
+def ltc_selective_scan(x, delta, A, B, C, D=None, z=None, delta_bias=None, state=None,
+                       cu_seqlens=None, delta_softplus=False):
+    """Selective state space scan -> (out, state_final). Of channel h and state n:
+
+        s_t = delta_t + delta_bias, or softplus of it with delta_softplus
+        v_t = exp(s_t A[h, n]) v_{t-1} + s_t B_t[n] x_t
+        out_t = (sum_n C_t[n] v_t + D x_t) silu(z_t)
+
+    x, delta, z  (B, T, H), float32, bfloat16 or float16, all alike; with cu_seqlens
+            (tokens, H). Without D, z or delta_bias their part is left out.
+    A       (H, N) float32, N <= 64; taken as it is: above 0, states may grow without bound
+    B, C    (B, T, N), or (B, T, G, N) for G groups of H / G neighbouring channels each,
+            x's type; with cu_seqlens (tokens, N) or (tokens, G, N)
+    D, delta_bias  (H,) float32
+    state   (B, H, N) float32, or None for zero
+    cu_seqlens  as in ltc_gated_scan; tokens outside all sequences give zeros, in out and
+            in the gradients, whatever they hold
+    out     x's shape and type; state_final (B, H, N) float32.
+
+    States and sums are float32. Gradients reach all inputs through both outputs; for the
+    backward the forward keeps every 16th state (H N floats).
+    """
+    return tuple(_require_ext().selective_scan(x, delta, A, B, C, D, z, delta_bias, state,
+                                               cu_seqlens, bool(delta_softplus)))
+
+
+def ltc_selective_scan_step(x, delta, A, B, C, state, D=None, z=None, delta_bias=None, slots=None,
+                            delta_softplus=False):
+    """One token of each stream: returns out (B, H) and updates `state` in place.
+
+    x, delta, z (B, H); B, C (B, N) or (B, G, N); state (B, H, N) float32, or with slots a
+    pool (P, H, N), as in ltc_gated_scan_step. No backward.
+    """
+    return _require_ext().selective_scan_step(x, delta, A, B, C, state, D, z, delta_bias, slots,
+                                              bool(delta_softplus))
+
+
+def ltc_embed(table, ids, scale=1.0):
+    """scale table[ids]: table (V, H), ids (...) int32 or int64 -> (..., H), table's type.
+
+    A negative id is a token that is not there: zeros, and no gradient. An id of V or more
+    gives NaN and no gradient. The gradient of the table is dense; each row sums its
+    tokens' in float32, in their order, and is rounded once: the same bits in every run.
+    """
+    return _require_ext().embed(table, ids, float(scale))
+
+
+def ltc_adjust_logits(logits, context=None, prompt_lens=None, repetition=1.0, frequency=0.0,
+                      presence=0.0, bias_ids=None, bias=None, mask=None):
+    """Logits (..., V) adjusted for the choice of the next token; a new tensor of their type.
+
+    In float32, of a token with logit x, in this order:
+      it occurs in the context:  x / repetition where x > 0, else x * repetition
+      it occurs c > 0 times behind the prompt:  x - frequency * c - presence
+      bias_ids names it:  plus its bias (the sum of them, where it is named twice)
+      the mask does not allow it:  -inf, whatever x is
+
+    context  (..., n) int32 or int64: the tokens before; entries outside 0 ... V-1 are not
+            there (padding)
+    prompt_lens  (...) int32: the first entries of the context that are the prompt; None: 0
+    repetition, frequency, presence  numbers, or float32 (...) for one of each row
+    bias_ids, bias  (..., K) int32 or int64, and float32; K <= 1024
+    mask    (..., ceil(V / 32)) int32: token v is allowed where bit v % 32 of word v // 32
+            is set
+    context, bias_ids, bias and mask may also be one row, (n,), for all rows of logits.
+    No backward: it raises where a gradient would be wanted.
+    """
+    def split(v, none):
+        return (v, none) if isinstance(v, torch.Tensor) else (None, float(v))
+    rep, rep0 = split(repetition, 1.0)
+    (freq, freq0), (pres, pres0) = split(frequency, 0.0), split(presence, 0.0)
+    return _require_ext().adjust_logits(logits, context, prompt_lens, rep, freq, pres, rep0, freq0,
+                                        pres0, bias_ids, bias, mask)
 
 
 def _detach_tree(obj):
