@@ -71,7 +71,7 @@ int check_conv_types(int x_type, int weight_type, int activation) {
 // ---------------------------------------------------------------------------
 // Selective scan
 // ---------------------------------------------------------------------------
-int ssm_args(ltc::SsmArgs* a, int B, int T, int H, int N, int G, int packed) {
+int ssm_args(ltc::SsmArgs* a, int B, int T, int H, int N, int G, int packed, bool bwd) {
   if (B < 0 || T < 0 || H < 1 || N < 1 || G < 1)
     return host_fail(LTC_EINVAL, "dimensions must satisfy B >= 0, T >= 0, H >= 1, N >= 1, G >= 1");
   if (H % G != 0) return host_fail(LTC_EINVAL, "H must be a multiple of G");
@@ -86,29 +86,28 @@ int ssm_args(ltc::SsmArgs* a, int B, int T, int H, int N, int G, int packed) {
   a->N = N;
   a->G = G;
   a->ntok = ntok;
-  ltc::ssm_plan(a, packed != 0);
+  ltc::ssm_plan(a, packed != 0, bwd);
   const long long items = a->lines * a->chunks, hn = (long long)H * N;
-  if (items > kMaxGroups / ((long long)G * a->hblocks) || ntok > kMaxGroups * 32 / ((long long)G * a->quads) ||
+  if (items > kMaxGroups / ((long long)G * a->hblocks) || ntok > kMaxGroups * 32 / ((long long)G * N) ||
       (a->lines + 1) > kMaxGroups * 256 / hn)
     return host_fail(LTC_EUNSUPPORTED, "problem too large");
   return LTC_OK;
 }
 
 long long saved_floats(const ltc::SsmArgs& a) {
-  return a.lines * a.chunks * (a.len / ltc::kSsmTokens) * a.H * a.N;
+  return a.lines * a.tiles * a.H * a.N;
 }
 
 void carve_ssm(Pieces& c, ltc::SsmArgs& a, bool bwd) {
   const long long items = a.lines * a.chunks, hn = (long long)a.H * a.N;
-  const long long bc = a.ntok * a.G * a.quads * 8;
-  a.bc = c.take<float>(bc);
   if (a.chunks > 1) {
     a.ends = c.take<float>(items * hn);
     a.sumd = c.take<float>(items * a.H);
     a.drops = c.take<int>(items);
   }
   if (bwd) {
-    a.part_bc = c.take<float>(a.hblocks * bc);
+    constexpr int E = ltc::kSsmBwdStates;
+    a.part_bc = c.take<float>(a.hblocks * a.ntok * a.G * ((a.N + E - 1) / E) * 2 * E);
     a.part_a = c.take<float>(items * hn);
     a.part_h = c.take<float>(items * 2 * a.H);
   }
@@ -249,12 +248,12 @@ int ltc_causal_conv_step(const void* x, long long sxb, const void* weight, const
 
 long long ltc_selective_scan_saved_floats(int B, int T, int H, int N, int G, int packed) {
   ltc::SsmArgs a{};
-  return ssm_args(&a, B, T, H, N, G, packed) == LTC_OK ? saved_floats(a) : -1;
+  return ssm_args(&a, B, T, H, N, G, packed, true) == LTC_OK ? saved_floats(a) : -1;
 }
 
 static long long ssm_bytes(int B, int T, int H, int N, int G, int packed, bool bwd) {
   ltc::SsmArgs a{};
-  if (ssm_args(&a, B, T, H, N, G, packed) != LTC_OK) return -1;
+  if (ssm_args(&a, B, T, H, N, G, packed, bwd) != LTC_OK) return -1;
   Pieces c{nullptr};
   carve_ssm(c, a, bwd);
   return c.off;
@@ -276,7 +275,7 @@ int ltc_selective_scan_forward(const void* x, long long sxb, long long sxt, cons
                                void* stream) {
   host_clear_error();
   ltc::SsmArgs a{};
-  int rc = ssm_args(&a, B, T, H, N, G, cu_seqlens != nullptr);
+  int rc = ssm_args(&a, B, T, H, N, G, cu_seqlens != nullptr, false);
   if (rc != LTC_OK) return rc;
   a.x = x, a.sxb = sxb, a.sxt = sxt;
   a.d = delta, a.sdb = sdb, a.sdt = sdt;
@@ -319,7 +318,7 @@ int ltc_selective_scan_backward(const void* x, long long sxb, long long sxt, con
                                 long long workspace_bytes, void* stream) {
   host_clear_error();
   ltc::SsmArgs a{};
-  int rc = ssm_args(&a, B, T, H, N, G, cu_seqlens != nullptr);
+  int rc = ssm_args(&a, B, T, H, N, G, cu_seqlens != nullptr, true);
   if (rc != LTC_OK) return rc;
   a.x = x, a.sxb = sxb, a.sxt = sxt;
   a.d = delta, a.sdb = sdb, a.sdt = sdt;
@@ -366,7 +365,7 @@ int ltc_selective_scan_step(const void* x, long long sx, const void* delta, long
                             int H, int N, int G, int P, void* out, void* stream) {
   host_clear_error();
   ltc::SsmArgs sizes{};
-  int rc = ssm_args(&sizes, B, 1, H, N, G, 0);
+  int rc = ssm_args(&sizes, B, 1, H, N, G, 0, false);
   if (rc != LTC_OK) return rc;
   if (!known_type(type)) return host_fail(LTC_EINVAL, "type must be LTC_F32, LTC_BF16 or LTC_F16");
   if ((rc = check_step_rows(B, P, slots)) != LTC_OK) return rc;

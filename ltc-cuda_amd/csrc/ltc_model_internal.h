@@ -67,7 +67,8 @@ hipError_t launch_conv_step(int x_type, int K, const ConvStepArgs& a, hipStream_
 // ---------------------------------------------------------------------------
 constexpr int kSsmStatesMax = 64;
 constexpr int kSsmTokens = 16;  // of a batch; a state is saved before every batch
-constexpr int kSsmWavesMin = 4, kSsmWavesMax = 8;
+constexpr int kSsmBwdStates = 2;  // of a wave
+constexpr int kSsmWavesMax = 8;
 
 struct SsmArgs {
   const void *x, *d, *z;  // z may be null
@@ -82,20 +83,18 @@ struct SsmArgs {
   int B, T, H, N, G;      // sequences, tokens of each (packed: of all), channels, states, groups
   long long ntok;         // tokens in all
   // plan
-  int quads;              // of the states
-  int waves, rounds;      // of a workgroup; quads of a wave
   int hblocks;            // blocks of 64 channels in a group
   int len, chunks;        // tokens of a chunk; chunks of a sequence (packed: of all tokens)
   long long lines;        // sequences that are cut into chunks each (packed: 1)
   // workspace
-  float* bc;              // [G][quads][ntok][8]: B and C of four states
-  float* ends;            // [lines*chunks][N][H]: what leaves a chunk, then what enters it
+  float* ends;            // [lines*chunks][H][N]: what leaves a chunk, then what enters it
   float* sumd;            // [lines*chunks][H]: sums of the step sizes
   int* drops;             // [lines*chunks]: whether what enters is lost in the chunk
-  float* part_bc;         // [hblocks][G][quads][ntok][8]
-  float* part_a;          // [lines*chunks][N][H]
+  float* part_bc;         // [hblocks][G][pairs of states][ntok][4]: of B, then C
+  float* part_a;          // [lines*chunks][H][N]
   float* part_h;          // [lines*chunks][2][H]: of D and of the bias
-  float* saved;           // [lines*chunks][len/16][N][H], or null
+  long long tiles;        // batches of a line
+  float* saved;           // [lines][tiles][H][N], or null
   void* out;              // (ntok,H)
   float* hf;              // (B,H,N)
   // backward
@@ -108,8 +107,8 @@ struct SsmArgs {
   float* gs;              // (B,H,N) or null
 };
 
-// The plan of a call from its sizes: fills in quads to lines.
-void ssm_plan(SsmArgs* a, bool packed);
+// The plan of a call from its sizes: fills in hblocks to lines, and tiles.
+void ssm_plan(SsmArgs* a, bool packed, bool bwd);
 hipError_t launch_ssm_fwd(int type, const SsmArgs& a, hipStream_t s);
 hipError_t launch_ssm_bwd(int type, const SsmArgs& a, hipStream_t s);
 
