@@ -132,11 +132,11 @@ hipError_t launch_ssm_step(int type, const SsmStepArgs& a, hipStream_t s);
 // Embedding
 // ---------------------------------------------------------------------------
 constexpr int kSortThreads = 1024;
-constexpr int kSortTile = 4 * kSortThreads;  // ids of a workgroup
+constexpr int kSortTile = kSortThreads;      // ids of a workgroup
 constexpr int kSortBitsMax = 10;             // of one pass
 // Tiles up to which a workgroup adds up the other tiles' counts itself.
 constexpr int kSortTilesDirect = 64;
-constexpr int kEmbedPiece = 64;              // sorted ids that are summed together
+constexpr int kEmbedPiece = 32;              // sorted ids that are summed together
 
 struct EmbedArgs {
   const void* table;  // (V,H), row stride st

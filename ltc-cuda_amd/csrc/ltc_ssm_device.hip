@@ -966,11 +966,23 @@ __global__ __launch_bounds__(kStepThreads) void ssm_step_kernel(SsmStepArgs p, i
   float* state = p.state + slot * p.ssp + (long long)ch * p.N + n0;
   Vec<float, kSE> h{}, A{};
   float bias = 0.f, skip = 0.f;
+  Vec<T, kSE> bm{}, cm{};
+  T x{}, d{}, z{};
+  const auto load = [&](int r) {
+    x = static_cast<const T*>(p.x)[r * p.sx + ch];
+    d = static_cast<const T*>(p.d)[r * p.sd + ch];
+    if (p.z != nullptr) z = static_cast<const T*>(p.z)[r * p.sz + ch];
+    if (n > 0) {
+      bm = load_vec<T, kSE>(static_cast<const T*>(p.Bm) + r * p.sbb + g * p.sbg + n0, n);
+      cm = load_vec<T, kSE>(static_cast<const T*>(p.Cm) + r * p.scb + g * p.scg + n0, n);
+    }
+  };
   if (in && live) {
     if (n > 0) {
       h = load_vec<float, kSE>(state, n);
       A = load_vec<float, kSE>(p.A + (long long)ch * p.N + n0, n);
     }
+    load(row);
     if (p.dbias != nullptr) bias = p.dbias[ch];
     if (p.D != nullptr) skip = p.D[ch];
   }
@@ -996,36 +1008,29 @@ __global__ __launch_bounds__(kStepThreads) void ssm_step_kernel(SsmStepArgs p, i
 #pragma unroll
   for (int e = 0; e < kSE; ++e) f[e] = h.get(e);
   auto step = [&](int r) {
-    float y = 0.f, x = 0.f;
-    if (in) {
-      x = value(static_cast<const T*>(p.x) + r * p.sx + ch);
-      float dt = value(static_cast<const T*>(p.d) + r * p.sd + ch) + bias;
-      if (p.softplus) dt = softplus(dt);
-      if (n > 0) {
-        const Vec<T, kSE> b = load_vec<T, kSE>(static_cast<const T*>(p.Bm) + r * p.sbb + g * p.sbg + n0, n);
-        const Vec<T, kSE> c = load_vec<T, kSE>(static_cast<const T*>(p.Cm) + r * p.scb + g * p.scg + n0, n);
+    const float xf = (float)x;
+    float y = 0.f, dt = (float)d + bias;
+    if (p.softplus) dt = softplus(dt);
 #pragma unroll
-        for (int e = 0; e < kSE; ++e)
-          if (e < n) {
-            f[e] = fmaf(exp2_of(dt * (A.get(e) * kLog2e)), f[e], dt * x * b.get(e));
-            y = fmaf(c.get(e), f[e], y);
-          }
+    for (int e = 0; e < kSE; ++e)
+      if (e < n) {
+        f[e] = fmaf(exp2_of(dt * (A.get(e) * kLog2e)), f[e], dt * xf * bm.get(e));
+        y = fmaf(cm.get(e), f[e], y);
       }
-    }
     for (int o = lanes / 2; o > 0; o /= 2) y += __shfl_xor(y, o);
     if (in && lane == 0) {
-      y = fmaf(skip, x, y);
-      if (p.z != nullptr) {
-        const float z = value(static_cast<const T*>(p.z) + r * p.sz + ch);
-        y *= z * sigmoid(z);
-      }
+      y = fmaf(skip, xf, y);
+      if (p.z != nullptr) y *= (float)z * sigmoid((float)z);
       out[(long long)r * p.H] = (T)y;
     }
   };
   step(row);
   if (more)
-    for (int r = row + 1; r < p.B; ++r)
-      if (p.slots[r] == slot) step(r);
+    for (int r = row + 1; r < p.B; ++r) {
+      if (p.slots[r] != slot) continue;
+      if (in) load(r);
+      step(r);
+    }
   if (in && n > 0) {
     h.put(f);
     store_vec<float, kSE>(state, h, n);

@@ -157,10 +157,16 @@ __device__ __forceinline__ void sort_tile(const EmbedArgs& p, SortShared& sh, in
 #pragma unroll
       for (int w = 0; w < SortShared::kWaves; ++w) total += sh.hist[w][d];
     } else if (direct) {
-      for (int t = 0; t < p.tiles; ++t) {
-        const unsigned c = p.counts[(long long)t * buckets + d];
-        if (t < tile) lower += c;
-        total += c;
+      constexpr int kAhead = 16;
+      for (int t0 = 0; t0 < p.tiles; t0 += kAhead) {
+        unsigned c[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) c[j] = p.counts[(long long)min(t0 + j, p.tiles - 1) * buckets + d];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          if (t0 + j < tile) lower += c[j];
+          if (t0 + j < p.tiles) total += c[j];
+        }
       }
     } else {
       lower = p.counts[(long long)tile * buckets + d];
@@ -262,15 +268,23 @@ __global__ __launch_bounds__(kThreads) void embed_piece_kernel(EmbedArgs p, int 
   store_vec<float, V>(p.sums + (long long)piece * p.H + c, o, n);
 }
 
-// Rows of the gradient, `lanes` threads to each.
+// Rows of the gradient, `lanes` threads to each. A row is a chain of loads, of its run's
+// ends, its places and its rows, so what counts is how many rows are at work at once: few
+// registers, and one row to a thread (four, their ends read together, took 162 us for
+// 92 at 65536 rows of 2048 bf16; a wave to a row 203).
 template <class T>
-__global__ __launch_bounds__(kThreads) void embed_rows_kernel(EmbedArgs p, int lanes) {
+__global__ __launch_bounds__(kThreads, 8) void embed_rows_kernel(EmbedArgs p, int lanes) {
   constexpr int V = 16 / (int)sizeof(T);
+  constexpr int kSums = 4;  // of pieces, under way together
   const int lane = threadIdx.x & (lanes - 1);
   const long long row = (long long)blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes;
   if (row >= p.V) return;
   const int* pos = p.pos[(p.passes - 1) & 1];
-  const int lo = p.n > 0 ? p.begin[row] : -1, hi = lo < 0 ? lo : p.end[row];
+  int lo = -1, hi = -1;
+  if (p.n > 0) {
+    lo = p.begin[row];
+    hi = p.end[row];  // of an id that does not occur, anything
+  }
   // whole pieces between, if any
   const int p0 = (lo + kEmbedPiece - 1) / kEmbedPiece, p1 = hi / kEmbedPiece;
   T* to = static_cast<T*>(p.gt) + row * p.H;
@@ -282,10 +296,18 @@ __global__ __launch_bounds__(kThreads) void embed_rows_kernel(EmbedArgs p, int l
         add_rows<T, V>(p, pos, lo, hi, c, n, f);
       } else {
         add_rows<T, V>(p, pos, lo, p0 * kEmbedPiece, c, n, f);
-        for (int i = p0; i < p1; ++i) {
-          const Vec<float, V> s = load_vec<float, V>(p.sums + (long long)i * p.H + c, n);
+        const float* sums = p.sums + c;
+        for (int i = p0; i < p1; i += kSums) {
+          Vec<float, V> s[kSums];
 #pragma unroll
-          for (int v = 0; v < V; ++v) f[v] += s.get(v);
+          for (int k = 0; k < kSums; ++k)
+            s[k] = load_vec<float, V>(sums + (long long)min(i + k, p1 - 1) * p.H, n);
+#pragma unroll
+          for (int k = 0; k < kSums; ++k)
+            if (i + k < p1) {
+#pragma unroll
+              for (int v = 0; v < V; ++v) f[v] += s[k].get(v);
+            }
         }
         add_rows<T, V>(p, pos, p1 * kEmbedPiece, hi, c, n, f);
       }
@@ -298,9 +320,9 @@ __global__ __launch_bounds__(kThreads) void embed_rows_kernel(EmbedArgs p, int l
   }
 }
 
-int row_lanes(int H, int V) {
+int row_lanes(int H, int V, int most) {
   int lanes = 1;
-  while (lanes < kThreads && lanes * V < H) lanes *= 2;
+  while (lanes < most && lanes * V < H) lanes *= 2;
   return lanes;
 }
 
@@ -333,7 +355,7 @@ __device__ __forceinline__ bool allowed(const int* mask, int v) { return mask[v 
 template <class T>
 __global__ __launch_bounds__(kThreads) void adjust_kernel(AdjustArgs p) {
   constexpr int V = 16 / (int)sizeof(T);
-  extern __shared__ unsigned count[];
+  extern __shared__ __attribute__((aligned(16))) unsigned count[];
   const long long row = blockIdx.x / (unsigned)p.segs;
   const int lo = (int)(blockIdx.x % (unsigned)p.segs) * p.seg;
   const int len = p.V - lo < p.seg ? p.V - lo : p.seg;
@@ -343,32 +365,60 @@ __global__ __launch_bounds__(kThreads) void adjust_kernel(AdjustArgs p) {
   const T* x = static_cast<const T*>(p.logits) + row * p.sl + lo;
   T* out = static_cast<T*>(p.out) + row * p.V + lo;
   const int* mask = p.mask != nullptr ? p.mask + row * p.sm + lo / 32 : nullptr;
+  // The first logits are under way while the context is counted.
+  constexpr int kAhead = 4;
+  Vec<T, V> r[kAhead];
+  const auto get = [&](int i) { return i < len ? load_vec<T, V>(x + i, len - i) : Vec<T, V>{}; };
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) r[j] = get((j * kThreads + (int)threadIdx.x) * V);
   if (p.ctx > 0) {
     for (int i = threadIdx.x; i < p.seg; i += kThreads) count[i] = 0;
     __syncthreads();
     const int prompt = p.prompt != nullptr ? p.prompt[row] : 0;
-    for (int i = threadIdx.x; i < p.ctx; i += kThreads) {
-      const long long id = id_at(p.context, p.ctx64, row * p.sc + i);
-      if (id < lo || id >= (long long)lo + len) continue;
-      atomicOr(&count[id - lo], kSeen);
-      if (i >= prompt) atomicAdd(&count[id - lo], 1u);
+    constexpr int kIds = 8;  // of a thread, under way together
+    for (int i0 = threadIdx.x; i0 < p.ctx; i0 += kIds * kThreads) {
+      long long id[kIds];
+#pragma unroll
+      for (int j = 0; j < kIds; ++j)
+        id[j] = id_at(p.context, p.ctx64, row * p.sc + min(i0 + j * kThreads, p.ctx - 1));
+#pragma unroll
+      for (int j = 0; j < kIds; ++j) {
+        const int i = i0 + j * kThreads;
+        if (i >= p.ctx || id[j] < lo || id[j] >= (long long)lo + len) continue;
+        atomicOr(&count[id[j] - lo], kSeen);
+        if (i >= prompt) atomicAdd(&count[id[j] - lo], 1u);
+      }
     }
     __syncthreads();
   }
-  for (int i = threadIdx.x * V; i < len; i += kThreads * V) {
-    const int n = len - i;
-    const Vec<T, V> r = load_vec<T, V>(x + i, n);
-    const unsigned bits = mask != nullptr ? (unsigned)mask[i >> 5] >> (i & 31) : ~0u;
-    float f[V];
+  for (int i0 = threadIdx.x * V; i0 < len; i0 += kAhead * kThreads * V) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      f[v] = r.get(v);
-      if (p.ctx > 0) f[v] = adjusted(f[v], count[i + v], rep, freq, pres);
-      if (!(bits >> v & 1)) f[v] = -__builtin_inff();
+    for (int j = 0; j < kAhead; ++j) {
+      const int i = i0 + j * kThreads * V;
+      if (i >= len) continue;
+      const unsigned bits = mask != nullptr ? (unsigned)mask[i >> 5] >> (i & 31) : ~0u;
+      float f[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) f[v] = r[j].get(v);
+      if (p.ctx > 0) {
+        unsigned c[V], any = 0;
+        __builtin_memcpy(c, __builtin_assume_aligned(count + i, 16), sizeof(c));
+#pragma unroll
+        for (int v = 0; v < V; ++v) any |= c[v];
+        if (any != 0) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) f[v] = adjusted(f[v], c[v], rep, freq, pres);
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (!(bits >> v & 1)) f[v] = -__builtin_inff();
+      Vec<T, V> o;
+      o.put(f);
+      store_vec<T, V>(out + i, o, len - i);
     }
-    Vec<T, V> o;
-    o.put(f);
-    store_vec<T, V>(out + i, o, n);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) r[j] = get(i0 + (kAhead + j) * kThreads * V);
   }
   if (p.K == 0) return;
   // The biased logits once more: an id's first entry takes all of its entries, in order.
@@ -404,7 +454,7 @@ hipError_t launch_embed_fwd(int type, const EmbedArgs& a, hipStream_t s) {
   if (a.n == 0) return hipSuccess;
   return with_type(type, [&](auto t) {
     using T = decltype(t);
-    const int lanes = row_lanes(a.H, 16 / (int)sizeof(T)), rows = kThreads / lanes;
+    const int lanes = row_lanes(a.H, 16 / (int)sizeof(T), kThreads), rows = kThreads / lanes;
     LTC_LAUNCH((embed_fwd_kernel<T>), dim3((unsigned)((a.n + rows - 1) / rows)), dim3(kThreads), 0, s, a, lanes);
     return hipGetLastError();
   });
@@ -432,7 +482,7 @@ hipError_t launch_embed_bwd(int type, const EmbedArgs& a, hipStream_t s) {
       const long long pieces = (a.n + kEmbedPiece - 1) / kEmbedPiece;
       LTC_LAUNCH((embed_piece_kernel<T>), dim3((unsigned)(pieces * cblocks)), dim3(kThreads), 0, s, a, cblocks);
     }
-    const int lanes = row_lanes(a.H, V), rows = kThreads / lanes;
+    const int lanes = row_lanes(a.H, V, kThreads), rows = kThreads / lanes;
     LTC_LAUNCH((embed_rows_kernel<T>), dim3((unsigned)(((long long)a.V + rows - 1) / rows)), dim3(kThreads), 0, s, a,
                lanes);
     return hipGetLastError();

@@ -82,7 +82,9 @@ def test_selective_scan(lib):
     sizes = [({"H": 0}, "H >= 1"), ({"N": 0}, "N >= 1"), ({"N": 65}, "64 states"), ({"G": 3}, "multiple"),
              ({"G": 0}, "G >= 1"), ({"B": -1}, "B >= 0"), ({"ty": 3}, "type"), ({"x": None}, "NULL"),
              ({"d": None}, "NULL"), ({"A": None}, "NULL"), ({"Bm": None}, "NULL"), ({"Cm": None}, "NULL")]
-    big = [({"B": INT_MAX - 1, "T": 2}, "too large"), ({"ws": None}, "too small"), ({"ws": 264}, "aligned")]
+    # long sequences of few channels are cut, and what enters the pieces is worked out
+    assert f.ltc_selective_scan_fwd_workspace_bytes(2, 400, 4, 2, 1, 0) > 0
+    big = [({"B": INT_MAX - 1, "T": 2}, "too large"), ({"ws": None, "T": 400}, "too small"), ({"ws": 264}, "aligned")]
     _refused(lib, fwd, sizes + big + [({"out": None}, "NULL"), ({"hf": None}, "state_final"),
                                       ({"save": 1}, "saved"), ({"T": -1}, "T >= 0")])
     _refused(lib, bwd, sizes + big + [({"saved": None}, "saved"), ({"gz": 1}, "grad_z")])
