@@ -22,7 +22,9 @@ this module's own CPU implementation of the same equations (the reference
 does the same, ltc.py:293-323).
 
 Beyond the reference: `LinearTimeConstant`, the layer without recurrent synapses, whose
-time axis is parallel, and `TokenReadout`, from states to token scores and losses.
+time axis is parallel; `TokenEmbedding`, `SelectiveTimeConstant` and `TokenReadout`, which
+make a model over tokens: rows of a table in, a layer whose time constants the input
+selects, token scores, losses and adjusted scores out.
 """
 
 from __future__ import annotations
@@ -515,13 +517,174 @@ class LinearTimeConstant(nn.Module):
         return out
 
 
+class TokenEmbedding(nn.Module):
+    """Rows of a table for tokens, times a scale: forward(ids (...)) -> (..., dim).
+
+    A negative id is a token that is not there: zeros, and no gradient. The table's
+    gradient is dense and the same bits in every run (ltc_cuda.ltc_embed). CPU tensors take
+    plain torch, which raises for an id past the vocabulary where the kernels give NaN.
+    """
+
+    def __init__(self, vocab: int, dim: int, scale: float = 1.0, dtype=None):
+        super().__init__()
+        self.scale = float(scale)
+        self.weight = nn.Parameter(torch.randn(vocab, dim, dtype=dtype) * dim ** -0.5)
+
+    def forward(self, ids):
+        if _on_hip(self.weight, ids):
+            return ltc_cuda.ltc_embed(self.weight, ids, self.scale)
+        there = (ids >= 0).unsqueeze(-1)
+        rows = F.embedding(ids.clamp(min=0).long(), self.weight) * self.scale
+        return torch.where(there, rows, torch.zeros_like(rows))
+
+
+def _causal_conv_plain(x, weight, bias, state, cu_seqlens=None):
+    """ltc_cuda.ltc_causal_conv with "silu" in plain torch."""
+    K = weight.shape[1]
+    if cu_seqlens is None:
+        line = torch.cat([state, x], 1)
+        y = sum(line[:, k:k + x.shape[1]] * weight[:, k] for k in range(K)) + bias
+        return F.silu(y), line[:, x.shape[1]:]
+    cu = cu_seqlens.tolist()
+    outs, tails = [x.new_zeros(cu[0], x.shape[1])], []
+    for s in range(len(cu) - 1):
+        o, t = _causal_conv_plain(x[None, cu[s]:cu[s + 1]], weight, bias, state[s:s + 1])
+        outs.append(o[0])
+        tails.append(t)
+    outs.append(x.new_zeros(x.shape[0] - cu[-1], x.shape[1]))
+    return torch.cat(outs), (torch.cat(tails) if tails else state)
+
+
+def _selective_scan_plain(x, delta, A, B, C, D, z, delta_bias, state, cu_seqlens=None):
+    """ltc_cuda.ltc_selective_scan with a softplus of the step sizes in plain torch."""
+    if cu_seqlens is None:
+        s = F.softplus(delta.float() + delta_bias)
+        h, outs = state, []
+        for t in range(x.shape[1]):
+            u = (s[:, t] * x[:, t].float()).unsqueeze(-1) * B[:, t, None].float()
+            h = torch.exp(s[:, t, :, None] * A) * h + u
+            y = (h * C[:, t, None].float()).sum(-1) + D * x[:, t].float()
+            outs.append((y * F.silu(z[:, t].float())).to(x.dtype))
+        return (torch.stack(outs, 1) if outs else torch.zeros_like(x)), h
+    cu = cu_seqlens.tolist()
+    outs, finals = [x.new_zeros(cu[0], x.shape[1])], []
+    for s in range(len(cu) - 1):
+        part = [v[None, cu[s]:cu[s + 1]] for v in (x, delta, B, C, z)]
+        o, h = _selective_scan_plain(part[0], part[1], A, part[2], part[3], D, part[4], delta_bias,
+                                     state[s:s + 1])
+        outs.append(o[0])
+        finals.append(h)
+    outs.append(x.new_zeros(x.shape[0] - cu[-1], x.shape[1]))
+    return torch.cat(outs), (torch.cat(finals) if finals else state)
+
+
+class SelectiveTimeConstant(nn.Module):
+    """Layer of states whose time constants the input selects: a projection to the channels
+    and their gates, a short causal convolution, a selective state space scan, and a
+    projection back.
+
+    Each channel h has `states` states v with v' = exp(s_t A) v + s_t B_t x_t, where the step
+    sizes s_t (softplus of a projection of rank `rank`), the drives B_t and the readouts C_t
+    all come from the input; LinearTimeConstant has one state a channel, whose decay comes
+    from its synapses.
+
+    forward(x (B, T, dim)) -> (out, state), or packed x (tokens, dim) with cu_seqlens as
+    ltc_cuda.ltc_gated_scan takes them. A state is a pair: the convolution's last inputs
+    (rows, taps-1, hidden) and the scan's states (rows, hidden, states) in float32;
+    new_state(rows) makes a zero one. step(x (B, dim), state, slots) serves streams token by
+    token, their state updated in place, in rows of a pool if slots are given. The
+    projections have no bias: torch forms its gradient with a reduction that a captured graph
+    replays wrongly (_ScaleColumns).
+    """
+
+    def __init__(self, dim: int, hidden: int | None = None, states: int = 16, taps: int = 4,
+                 rank: int | None = None, dt_min: float = 1e-3, dt_max: float = 0.1, dtype=None):
+        super().__init__()
+        hidden = 2 * dim if hidden is None else hidden
+        rank = max(1, dim // 16) if rank is None else rank
+        self.dim, self.hidden, self.states, self.taps, self.rank = dim, hidden, states, taps, rank
+        self.in_proj = nn.Linear(dim, 2 * hidden, bias=False, dtype=dtype)
+        self.x_proj = nn.Linear(hidden, rank + 2 * states, bias=False, dtype=dtype)
+        self.dt_proj = nn.Linear(rank, hidden, bias=False, dtype=dtype)
+        self.out_proj = nn.Linear(hidden, dim, bias=False, dtype=dtype)
+        self.conv_weight = nn.Parameter((torch.rand(hidden, taps) * 2 - 1) * taps ** -0.5)
+        self.conv_bias = nn.Parameter(torch.zeros(hidden))
+        # decays of 1 to `states` of a step, steps spread over their range in logarithm
+        self.A_log = nn.Parameter(torch.log(torch.arange(1, states + 1).float()).repeat(hidden, 1))
+        self.D = nn.Parameter(torch.ones(hidden))
+        lo, hi = torch.tensor(dt_min).log(), torch.tensor(dt_max).log()
+        dt = torch.exp(lo + (hi - lo) * torch.rand(hidden))
+        self.dt_bias = nn.Parameter(dt + torch.log(-torch.expm1(-dt)))
+
+    def new_state(self, rows: int):
+        w = self.in_proj.weight
+        return (w.new_zeros(rows, self.taps - 1, self.hidden),
+                torch.zeros(rows, self.hidden, self.states, device=w.device))
+
+    def _rates(self):
+        """What the scan takes in float32, whatever the module's type."""
+        return -torch.exp(self.A_log.float()), self.D.float(), self.dt_bias.float()
+
+    def _selected(self, u):
+        """Step sizes, drives and readouts of the convolved input."""
+        r, n = self.rank, self.states
+        low = self.x_proj(u)
+        return self.dt_proj(low[..., :r]), low[..., r:r + n], low[..., r + n:]
+
+    def forward(self, x, state=None, cu_seqlens=None):
+        x = x.to(self.in_proj.weight.dtype)
+        both = self.in_proj(x)
+        u, z = both[..., :self.hidden], both[..., self.hidden:]
+        A, D, dt_bias = self._rates()
+        tail, h = (None, None) if state is None else state
+        if _on_hip(x, tail, h, cu_seqlens):
+            u, tail = ltc_cuda.ltc_causal_conv(u, self.conv_weight, self.conv_bias, tail, cu_seqlens, "silu")
+            delta, B, C = self._selected(u)
+            y, h = ltc_cuda.ltc_selective_scan(u, delta, A, B, C, D, z, dt_bias, h, cu_seqlens, True)
+        else:
+            if state is None:
+                tail, h = self.new_state(x.shape[0] if cu_seqlens is None else cu_seqlens.numel() - 1)
+            u, tail = _causal_conv_plain(u, self.conv_weight, self.conv_bias, tail, cu_seqlens)
+            u = u.to(x.dtype)
+            delta, B, C = self._selected(u)
+            y, h = _selective_scan_plain(u, delta, A, B, C, D, z, dt_bias, h, cu_seqlens)
+        return self.out_proj(y), (tail, h)
+
+    @torch.no_grad()
+    def step(self, x, state, slots=None):
+        """One token of each stream: x (B, dim) -> (B, dim); `state` is updated in place.
+        A negative slot is padding: zeros."""
+        x = x.to(self.in_proj.weight.dtype)
+        both = self.in_proj(x)
+        u, z = both[..., :self.hidden], both[..., self.hidden:]
+        A, D, dt_bias = self._rates()
+        tail, h = state
+        if _on_hip(x, tail, h, slots):
+            u = ltc_cuda.ltc_causal_conv_step(u, self.conv_weight, tail, self.conv_bias, slots, "silu")
+            delta, B, C = self._selected(u)
+            y = ltc_cuda.ltc_selective_scan_step(u, delta, A, B, C, h, D, z, dt_bias, slots, True)
+            return self.out_proj(y)
+        out = torch.zeros_like(x)
+        for b in range(x.shape[0]):
+            s = b if slots is None else int(slots[b])
+            if s < 0:
+                continue
+            ub, tail[s:s + 1] = _causal_conv_plain(u[b, None, None], self.conv_weight, self.conv_bias, tail[s:s + 1])
+            ub = ub.to(x.dtype)
+            delta, B, C = self._selected(ub)
+            y, h[s:s + 1] = _selective_scan_plain(ub, delta, A, B, C, D, z[b, None, None], dt_bias, h[s:s + 1])
+            out[b] = self.out_proj(y)[0, 0]
+        return out
+
+
 class TokenReadout(nn.Module):
     """Linear readout of a layer's states to the logits of a vocabulary, and what is
     asked of them: scores of given tokens, and a teacher's distribution to learn.
 
     forward(h) -> logits; log_probs(h, ids) -> ltc_cuda.ltc_token_logprobs of them;
     distill(h, teacher_logits, teacher_ids) -> ltc_cuda.ltc_top_distill's loss of each
-    row. The logits are in the readout's own type (float32, bfloat16 or float16), what
+    row; adjusted(h, context, ...) -> the logits as ltc_cuda.ltc_adjust_logits leaves them
+    for the choice of the next token. The logits are in the readout's own type (float32, bfloat16 or float16), what
     is made of them in float32. There is no bias: torch forms its gradient with a
     reduction that a captured graph replays wrongly (_ScaleColumns). CPU tensors take
     plain torch, which raises for an id past the vocabulary where the kernels give NaN.
@@ -565,3 +728,40 @@ class TokenReadout(nn.Module):
         diff = lp - lq.gather(-1, teacher_ids.clamp(min=0).long())
         return temperature ** 2 * torch.where(p > 0, p * diff, torch.zeros_like(p)).sum(-1)
 
+    @torch.no_grad()
+    def adjusted(self, h, context=None, prompt_lens=None, repetition=1.0, frequency=0.0,
+                 presence=0.0, bias_ids=None, bias=None, mask=None):
+        """Logits with penalties for the context's tokens, biases and a grammar's mask."""
+        logits = self(h)
+        if _on_hip(logits):
+            return ltc_cuda.ltc_adjust_logits(logits, context, prompt_lens, repetition, frequency,
+                                              presence, bias_ids, bias, mask)
+        lead, V = logits.shape[:-1], logits.shape[-1]
+        v = logits.float().reshape(-1, V)
+
+        def rows(t):
+            t = t if t.dim() == len(lead) + 1 else t.expand(*lead, t.shape[-1])
+            return t.reshape(v.shape[0], -1)
+
+        def column(p):
+            return p.reshape(-1, 1) if isinstance(p, torch.Tensor) else p
+
+        if context is not None:
+            ids = rows(context)
+            there = (ids >= 0) & (ids < V)
+            start = 0 if prompt_lens is None else prompt_lens.reshape(-1, 1)
+            later = there & (torch.arange(ids.shape[1]) >= start)
+            at = ids.clamp(0, V - 1).long()
+            seen = torch.zeros_like(v).scatter_add_(1, at, there.float()) > 0
+            count = torch.zeros_like(v).scatter_add_(1, at, later.float())
+            rep = column(repetition)
+            v = torch.where(seen, torch.where(v > 0, v / rep, v * rep), v)
+            v = torch.where(count > 0, v - column(frequency) * count - column(presence), v)
+        if bias_ids is not None:
+            ids, b = rows(bias_ids), rows(bias)
+            there = (ids >= 0) & (ids < V)
+            v = v.scatter_add(1, ids.clamp(0, V - 1).long(), torch.where(there, b, torch.zeros_like(b)))
+        if mask is not None:
+            t = torch.arange(V)
+            v = v.masked_fill((rows(mask)[:, t // 32] >> (t % 32)) & 1 == 0, -float("inf"))
+        return v.to(logits.dtype).view(*lead, V)
