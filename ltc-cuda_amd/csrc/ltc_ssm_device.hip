@@ -7,14 +7,20 @@
 //   dL/dx = D s1 + skip dy        dL/dD = x s1 + sum_n A a h_{t-1} d
 //   dL/dA = sum_t D a h_{t-1} d
 //
-// Arithmetic bounds it: forward a product, an exponential (four times a product's time), a
-// product and two multiply-adds a state; backward these once more and about twelve. A
-// workgroup has 64 channels, one to a lane, and walks a chunk of the time axis in batches
-// of 16 tokens; its waves share the states, four to a wave. So B_t and C_t, the same for
-// all lanes, come through the scalar unit, from a copy that a small launch lays out; step
-// sizes are formed once, by one wave each, and handed round in shared memory; and so are
-// the waves' parts of the sums over states. The sums over channels, for dB and dC, are
-// formed by halving: 64 sums over 64 lanes take 63 exchanges instead of 384.
+// Arithmetic bounds it: forward a product, an exponential (twice a product's time), a
+// product and two multiply-adds a state; backward these once more and about twelve, and what
+// it takes to sum over channels. A product with a scalar or a lane-crossing operand takes
+// 4.4 cycles, one of a lane's own registers 2.4 if another wave shares the SIMD, and one
+// wave alone issues one in 4.4: measured.
+//
+// The forward gives a channel four lanes, each with four states, so waves need nothing of
+// one another. The backward gives it one lane of each of eight waves, each with two states;
+// step sizes are formed once and handed round in shared memory, the waves' sums over states
+// go the same way, and the sums over channels, for dB and dC, are formed by halving: 64
+// sums over 64 lanes take 63 exchanges instead of 384. (The backward with four lanes a
+// channel was built too: 837 us for 787 at B8 T2048 H2048 N16, since its decays, states and
+// sums need 370 registers.) Both walk a chunk of the time axis in batches of 16 tokens, the
+// next batch's inputs under way.
 //
 // The forward leaves the states before every batch for the backward. Sequences that are
 // too few to fill the chip are cut into chunks: a first launch runs each chunk from
@@ -226,11 +232,10 @@ __device__ __forceinline__ void back(F&& f) {
   each<kL>([&](auto i) { f(std::integral_constant<int, kL - 1 - decltype(i)::value>{}); });
 }
 
-// B and C of a batch and a wave's E states. They are the same for all lanes, which cost
-// nothing to hold them: each row of 16 lanes has all of them in kL * 2 E / 16 registers, and
-// instructions take them from a lane of the row (as a scalar operand would be taken, and
-// without the scalar cache's misses, which stood for 6 of 7 us of a batch). A token's 2 E
-// values lie side by side.
+// B and C of a batch and a wave's E states. They are the same for all lanes, so each row of
+// 16 lanes holds all of them in kL * 2 E / 16 registers, and instructions take them from a
+// lane of the row: as fast as a scalar operand, with no scalar loads to wait for. A token's
+// 2 E values lie side by side.
 template <class T, int E>
 struct Coeffs {
   static constexpr int kToken = 2 * E, kTokens = 16 / kToken, kRegs = kL / kTokens;

@@ -96,12 +96,18 @@ __global__ __launch_bounds__(kSortThreads) void embed_count_kernel(EmbedArgs p, 
 __global__ __launch_bounds__(64) void embed_scan_kernel(EmbedArgs p) {
   const int buckets = 1 << p.bits, d = blockIdx.x * 64 + threadIdx.x;
   if (d >= buckets) return;
+  constexpr int kAhead = 32;  // under way together
   unsigned sum = 0;
-  for (int t = 0; t < p.tiles; ++t) {
-    const long long at = (long long)t * buckets + d;
-    const unsigned c = p.counts[at];
-    p.counts[at] = sum;
-    sum += c;
+  for (int t0 = 0; t0 < p.tiles; t0 += kAhead) {
+    unsigned c[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) c[j] = p.counts[(long long)min(t0 + j, p.tiles - 1) * buckets + d];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (t0 + j >= p.tiles) break;
+      p.counts[(long long)(t0 + j) * buckets + d] = sum;
+      sum += c[j];
+    }
   }
   p.counts[(long long)p.tiles * buckets + d] = sum;
 }
