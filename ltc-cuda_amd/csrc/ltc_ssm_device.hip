@@ -120,44 +120,13 @@ struct Work {
   }
 };
 
-// Which of a batch's tokens begin a sequence, end one, and lie in one.
-struct Edges {
-  unsigned start, end, valid;
-  // Of the batch at t; q is the sequence that was met last.
-  __device__ __forceinline__ void find(const SsmArgs& p, int t, int c1, Seq& q) {
-    start = end = valid = 0;
-    const int n = c1 - t < kL ? c1 - t : kL;
-    int i = 0;
-    while (i < n) {
-      if (t + i < q.lo || t + i >= q.hi) q = seq_of(p.cu, p.B, p.T, (int)p.ntok, t + i, 0, 0);
-      const int m = q.hi - t < n ? q.hi - t : n;
-      if (q.s >= 0) {
-        if (q.lo == t + i) start |= 1u << i;
-        if (q.hi - t <= n) end |= 1u << (q.hi - t - 1);
-        valid |= ((1u << m) - 1) & ~((1u << i) - 1);
-      }
-      i = m;
-    }
-  }
-  // The tokens of the first sequence in `rest`, which holds valid tokens, and of the last.
-  __device__ __forceinline__ unsigned first(unsigned rest) const {
-    const unsigned from = rest & (0u - rest);
-    const unsigned more = (rest & start & ~from) | (~valid & ~(from - 1)) | (1u << kL);
-    return ((more & (0u - more)) - 1) & ~(from - 1);
-  }
-  __device__ __forceinline__ unsigned last(unsigned rest) const {
-    const unsigned upto = (2u << (31 - __clz((int)rest))) - 1;
-    const unsigned begins = upto & start, gaps = upto & ~valid;
-    const unsigned lo = begins != 0 ? 1u << (31 - __clz((int)begins)) : 0u;
-    const unsigned gap = gaps != 0 ? 2u << (31 - __clz((int)gaps)) : 0u;
-    const unsigned from = lo > gap ? lo : gap;
-    return from == 0 ? upto : upto & ~(from - 1);
-  }
-};
+using Edges = EdgesOf<kL>;
 __device__ __forceinline__ int lowest(unsigned m) { return __ffs((int)m) - 1; }
 __device__ __forceinline__ int highest(unsigned m) { return 31 - __clz((int)m); }
-__device__ __forceinline__ long long state_at(const SsmArgs& p, int t) {
-  return (long long)seq_of(p.cu, p.B, p.T, (int)p.ntok, t, 0, 0).s * p.H * p.N;
+// Calls f with the offset of the states of the sequence that token t begins or ends.
+template <class F>
+__device__ __forceinline__ void at_state(const SsmArgs& p, int t, F&& f) {
+  at_edge(p.cu, p.B, p.T, (int)p.ntok, t, [&](int s) { f((long long)s * p.H * p.N); });
 }
 
 // The E states from the q-th E of a lane's channel in (rows,H,N), n of them there.
@@ -173,8 +142,7 @@ __device__ __forceinline__ void read_states(const SsmArgs& p, const Work& w, int
 #pragma unroll
   for (int e = 0; e < E; ++e) h[e] = 0.f;
   if (from == nullptr) return;
-  const long long s = state_at(p, t);
-  states<E>(p, w, q, [&](int e, long long at) { h[e] = from[s + at]; });
+  at_state(p, t, [&](long long s) { states<E>(p, w, q, [&](int e, long long at) { h[e] = from[s + at]; }); });
 #pragma unroll
   for (int e = 0; e < E; ++e) settle(h[e]);
 }
@@ -425,7 +393,7 @@ __global__ __launch_bounds__(64 * kFWaves) void ssm_fwd_kernel(SsmArgs p) {
   Seq seq{-1, 0, 0, 0};
   for (int t = w.c0; t < w.c1; t += kL) {
     Edges ed;
-    ed.find(p, t, w.c1, seq);
+    ed.find(p.cu, p.B, p.T, (int)p.ntok, t, w.c1, seq);
     float dt[kFOwn], u[kFOwn];
 #pragma unroll
     for (int j = 0; j < kFOwn; ++j) {
@@ -476,8 +444,9 @@ __global__ __launch_bounds__(64 * kFWaves) void ssm_fwd_kernel(SsmArgs p) {
           if (r == 0) y[i] = 0.f;
           if (EDGE && !(ed.valid >> i & 1)) return;
           if (EDGE && (ed.start >> i & 1)) {
-            const long long s = state_at(p, t + i);
-            get(p.h0 != nullptr ? p.h0 + s : nullptr, r, h[r]);
+            const float* from = nullptr;
+            if (p.h0 != nullptr) at_state(p, t + i, [&](long long s) { from = p.h0 + s; });
+            get(from, r, h[r]);
             if (i == 0 && !STATE && p.saved != nullptr)
               put(p.saved + (w.b * p.tiles + (t - w.first) / kL) * HN, r, h[r]);
           }
@@ -490,7 +459,7 @@ __global__ __launch_bounds__(64 * kFWaves) void ssm_fwd_kernel(SsmArgs p) {
             if (!STATE) part_y = e == 0 ? k.C(e, n) * h[r][e] : fmaf(k.C(e, n), h[r][e], part_y);
           }
           if (!STATE) y[i] = r == 0 ? part_y : y[i] + part_y;
-          if (!STATE && EDGE && (ed.end >> i & 1)) put(p.hf + state_at(p, t + i), r, h[r]);
+          if (!STATE && EDGE && (ed.end >> i & 1)) at_state(p, t + i, [&](long long s) { put(p.hf + s, r, h[r]); });
         });
       });
     };
@@ -623,7 +592,7 @@ ssm_bwd_state_kernel(SsmArgs p) {
   int buf = 0;
   for (int t = last; t >= w.c0; t -= kL, buf ^= 1) {
     Edges ed;
-    ed.find(p, t, w.c1, seq);
+    ed.find(p.cu, p.B, p.T, (int)p.ntok, t, w.c1, seq);
     if (t > w.c0) load(t - kL, next, bc_next);
 #pragma unroll
     for (int j = 0; j < kBMine; ++j) {
@@ -740,7 +709,7 @@ __global__ __launch_bounds__(64 * kSsmWavesMax) void ssm_bwd_kernel(SsmArgs p) {
   Seq seq{-1, 0, 0, 0};
   for (int t = last; t >= w.c0; t -= kL) {
     Edges ed;
-    ed.find(p, t, w.c1, seq);
+    ed.find(p.cu, p.B, p.T, (int)p.ntok, t, w.c1, seq);
     if (t > w.c0) load(t - kL, next, hnext, bc_next);
 #pragma unroll
     for (int j = 0; j < kBMine; ++j) {
@@ -821,10 +790,10 @@ __global__ __launch_bounds__(64 * kSsmWavesMax) void ssm_bwd_kernel(SsmArgs p) {
           }
         });
         if (seg & ed.start) {
-          if (p.gs != nullptr) {
-            const long long s = state_at(p, t + lowest(seg));
-            states<kBE>(p, w, q, [&](int e, long long at) { p.gs[s + at] = g[r][e]; });
-          }
+          if (p.gs != nullptr)
+            at_state(p, t + lowest(seg), [&](long long s) {
+              states<kBE>(p, w, q, [&](int e, long long at) { p.gs[s + at] = g[r][e]; });
+            });
 #pragma unroll
           for (int e = 0; e < kBE; ++e) g[r][e] = 0.f;
         }

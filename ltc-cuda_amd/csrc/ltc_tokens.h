@@ -48,4 +48,44 @@ __device__ __forceinline__ void span_of(const int* cu, int T, int N, int s, int&
   }
 }
 
+// Which of a batch's L tokens begin a sequence, end one, and lie in one.
+template <int L>
+struct EdgesOf {
+  unsigned start, end, valid;
+  // Of the batch at t, up to c1; q is the sequence that was met last.
+  __device__ __forceinline__ void find(const int* cu, int S, int T, int N, int t, int c1, Seq& q) {
+    start = end = valid = 0;
+    const int n = c1 - t < L ? c1 - t : L;
+    int i = 0;
+    while (i < n) {
+      if (t + i < q.lo || t + i >= q.hi) q = seq_of(cu, S, T, N, t + i, 0, 0);
+      const int m = q.hi - t < n ? q.hi - t : n;
+      if (q.s >= 0) {
+        if (q.lo == t + i) start |= 1u << i;
+        if (q.hi - t <= n) end |= 1u << (q.hi - t - 1);
+        valid |= ((1u << m) - 1) & ~((1u << i) - 1);
+      }
+      i = m;
+    }
+  }
+  // The tokens of the last sequence in `rest`, which holds valid tokens.
+  __device__ __forceinline__ unsigned last(unsigned rest) const {
+    const unsigned upto = (2u << (31 - __builtin_clz(rest))) - 1;
+    const unsigned begins = upto & start, gaps = upto & ~valid;
+    const unsigned lo = begins != 0 ? 1u << (31 - __builtin_clz(begins)) : 0u;
+    const unsigned gap = gaps != 0 ? 2u << (31 - __builtin_clz(gaps)) : 0u;
+    const unsigned from = lo > gap ? lo : gap;
+    return from == 0 ? upto : upto & ~(from - 1);
+  }
+};
+
+// Calls f with the sequence that token t begins or ends. An edge may have been found by the
+// search of another of its sequence's tokens; where boundaries are out of order the search
+// of t can end elsewhere, also outside all sequences. Then there is no state, and no call.
+template <class F>
+__device__ __forceinline__ void at_edge(const int* cu, int S, int T, int N, int t, F&& f) {
+  const int s = seq_of(cu, S, T, N, t, 0, 0).s;
+  if (s >= 0) f(s);
+}
+
 }  // namespace ltc

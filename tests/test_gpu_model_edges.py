@@ -1,0 +1,58 @@
+"""The convolution and the selective scan where their inputs are at an edge of what is
+allowed: boundaries of packed sequences in any order."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import ltc_cuda
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+ODD_BOUNDARIES = [[0, 40, 20, 64], [-5, 10, 64], [0, 10, 1000], [70, 80, 90], [64, 0], [2 ** 31 - 1, -2 ** 31],
+                  [0, 10, 3, 0], [3, 1, -3], [0, 33, 17, 0, 0], [50, 64, 5, 64, 0, 70]]
+
+
+@pytest.mark.parametrize("cu", ODD_BOUNDARIES)
+@pytest.mark.parametrize("T,N", [(64, 4), (200, 24)])
+def test_boundaries_out_of_order_or_range_stay_in_bounds(cu, T, N):
+    """Unspecified results, but no access out of range: whole calls, and a C call whose
+    states lie between others."""
+    g = torch.Generator().manual_seed(1)
+    c = torch.tensor(cu, dtype=torch.int32, device=DEV)
+    S, H = len(cu) - 1, 6
+
+    def leaf(*shape):
+        return torch.randn(*shape, generator=g).to(DEV).requires_grad_(True)
+
+    x, w, b, tail = leaf(T, H), leaf(H, 4), leaf(H), leaf(S, 3, H)
+    out, hf = ltc_cuda.ltc_causal_conv(x, w, b, tail, c, "silu")
+    grads = torch.autograd.grad([out, hf], [x, w, b, tail], [torch.ones_like(out), torch.ones_like(hf)])
+    assert out.shape == x.shape and hf.shape == tail.shape and grads[3].shape == tail.shape
+    delta, B, C, state = leaf(T, H), leaf(T, N), leaf(T, N), leaf(S, H, N)
+    A = (-torch.rand(H, N, generator=g)).to(DEV).requires_grad_(True)
+    leaves = [x, delta, A, B, C, state]
+    out, hf = ltc_cuda.ltc_selective_scan(x, delta, A, B, C, state=state, cu_seqlens=c, delta_softplus=True)
+    grads = torch.autograd.grad([out, hf], leaves, [torch.ones_like(out), torch.ones_like(hf)])
+    assert out.shape == x.shape and hf.shape == state.shape and grads[5].shape == state.shape
+    # final states and the initial ones' gradients between 64 rows of others
+    lib = ltc_cuda._cuda_module.capi.lib
+    sizes = (S, T, H, N, 1, 1)
+    row = H * N
+    around = torch.full((2, S + 128, row), 7.0, device=DEV)
+    ends = [around[k, 64:64 + S].data_ptr() for k in range(2)]
+    o, saved = torch.empty(T, H, device=DEV), torch.empty(lib.ltc_selective_scan_saved_floats(*sizes), device=DEV)
+    need = max(lib.ltc_selective_scan_fwd_workspace_bytes(*sizes), lib.ltc_selective_scan_bwd_workspace_bytes(*sizes))
+    ws = torch.empty(need + 256, dtype=torch.uint8, device=DEV)
+    at = (ws.data_ptr() + 255) // 256 * 256
+    ins = (x.data_ptr(), 0, H, delta.data_ptr(), 0, H, A.data_ptr(), B.data_ptr(), 0, N, 0, C.data_ptr(), 0, N, 0,
+           None, None, 0, 0, None, state.data_ptr(), c.data_ptr(), 0, 1, S, T, H, N, 1)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.ltc_selective_scan_forward(*ins, 1, o.data_ptr(), ends[0], saved.data_ptr(), at, need, stream) == 0
+    ones, gh = torch.ones(T, H, device=DEV), torch.ones(S, H, N, device=DEV)
+    assert lib.ltc_selective_scan_backward(*ins, saved.data_ptr(), ones.data_ptr(), 0, H, gh.data_ptr(), None, None,
+                                           None, None, None, None, None, None, ends[1], at, need, stream) == 0
+    torch.cuda.synchronize()
+    assert bool((around[:, :64] == 7).all()) and bool((around[:, 64 + S:] == 7).all())
