@@ -747,10 +747,12 @@ __global__ __launch_bounds__(64 * kSsmWavesMax) void ssm_bwd_kernel(SsmArgs p) {
         const int q = r * waves + w.wave;
         if (NG > 1 && q >= pairs) return;
         bc[r].arrive(p, w, q, seg);
-        // the batch's decays and the states before its tokens once more
+        // the batch's decays and the states before its tokens once more; a lane without a
+        // channel has read another group's, and its part in the sums over channels has to
+        // be zero whatever they are
         float a[kL][kBE], hp[kL][kBE], h[kBE];
 #pragma unroll
-        for (int e = 0; e < kBE; ++e) h[e] = hin[r][e];
+        for (int e = 0; e < kBE; ++e) h[e] = w.in ? hin[r][e] : 0.f;
         if (seg & ed.start & ~1u) read_states<kBE>(p, w, q, p.h0, t + lowest(seg), h);
         each<kL>([&](auto i_) {
           constexpr int i = decltype(i_)::value;

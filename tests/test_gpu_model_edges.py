@@ -1,11 +1,12 @@
 """The convolution and the selective scan where their inputs are at an edge of what is
-allowed: boundaries of packed sequences in any order."""
+allowed: boundaries of packed sequences in any order, channels that are not finite."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
+import _model_ref as R
 import ltc_cuda
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +57,46 @@ def test_boundaries_out_of_order_or_range_stay_in_bounds(cu, T, N):
                                            None, None, None, None, None, None, ends[1], at, need, stream) == 0
     torch.cuda.synchronize()
     assert bool((around[:, :64] == 7).all()) and bool((around[:, 64 + S:] == 7).all())
+
+
+@pytest.mark.parametrize("H,G,N,dtype", [(10, 2, 16, "fp32"), (10, 2, 24, "bf16"), (140, 2, 5, "fp32"),
+                                         (195, 3, 40, "fp16")])
+@pytest.mark.parametrize("T,cu", [(40, None), (200, None), (200, [0, 30, 190])])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_a_channel_that_is_not_finite_stays_in_its_group(H, G, N, dtype, T, cu, bad):
+    """Groups that do not fill blocks of 64 channels: the first channel's state and inputs
+    are in the gradients of its own group's B and C, and in no other's."""
+    g = torch.Generator().manual_seed(2)
+    dt, lead = R.TYPES[dtype], (T,) if cu else (1, T)
+    rows = len(cu) - 1 if cu else 1
+
+    def rand(*shape, t=dt):
+        return torch.randn(*shape, generator=g).to(t).to(DEV)
+
+    t = {"x": rand(*lead, H), "delta": rand(*lead, H), "A": -rand(H, N, t=torch.float32).abs(),
+         "B": rand(*lead, G, N), "C": rand(*lead, G, N), "D": rand(H, t=torch.float32), "z": rand(*lead, H),
+         "state": rand(rows, H, N, t=torch.float32)}
+    go, gh = rand(*lead, H), rand(rows, H, N, t=torch.float32)
+    c = None if cu is None else torch.tensor(cu, dtype=torch.int32, device=DEV)
+
+    def run(kw):
+        kw = {k: v.clone().requires_grad_(True) for k, v in kw.items()}
+        out, hf = ltc_cuda.ltc_selective_scan(**kw, cu_seqlens=c, delta_softplus=True)
+        return out, hf, dict(zip(kw, torch.autograd.grad([out, hf], list(kw.values()), [go, gh])))
+
+    out, hf, grads = run(t)
+    for name in ("state", "x"):
+        kw = {k: v.clone() for k, v in t.items()}
+        if name == "state":
+            kw["state"][:, 0] = bad
+        else:
+            kw["x"][..., 0] = bad
+        o, h, got = run(kw)
+        assert not bool(o[..., 0].isfinite().all())
+        assert torch.equal(o[..., 1:], out[..., 1:]) and torch.equal(h[:, 1:], hf[:, 1:])
+        for k in ("B", "C"):
+            assert torch.equal(got[k][..., 1:, :], grads[k][..., 1:, :]), (name, k)
+        for k in ("x", "delta", "z"):
+            assert torch.equal(got[k][..., 1:], grads[k][..., 1:]), (name, k)
+        assert torch.equal(got["A"][1:], grads["A"][1:]) and torch.equal(got["D"][1:], grads["D"][1:])
+        assert torch.equal(got["state"][:, 1:], grads["state"][:, 1:])
