@@ -492,6 +492,14 @@ __global__ __launch_bounds__(64 * kFWaves) void ssm_fwd_kernel(SsmArgs p) {
   }
 }
 
+// exp2(x) v + e. Where the exponential alone would leave the range its whole powers of two
+// are applied last: a v of zero stays zero, a small one becomes what it is by definition.
+__device__ __forceinline__ float joined(float x, float v, float e) {
+  if (!(x > 126.f)) return fmaf(exp2_of(x), v, e);
+  const float whole = rintf(x);
+  return ldexpf(exp2_of(x - whole) * v, (int)fminf(whole, 1024.f)) + e;
+}
+
 // What enters each chunk, from what leaves the chunks before it, in their order (backward:
 // after it, from the last).
 template <bool BWD>
@@ -520,7 +528,7 @@ __global__ __launch_bounds__(256) void ssm_carry_kernel(SsmArgs p) {
       if (j0 + k >= p.chunks) break;
       const long long c = line * p.chunks + (BWD ? p.chunks - 1 - j0 - k : j0 + k);
       p.ends[c * hn + at] = carry;
-      carry = lost[k] ? e[k] : fmaf(exp2_of(A2 * d[k]), carry, e[k]);
+      carry = lost[k] ? e[k] : joined(A2 * d[k], carry, e[k]);
     }
   }
 }

@@ -1,5 +1,6 @@
 """The convolution and the selective scan where their inputs are at an edge of what is
-allowed: boundaries of packed sequences in any order, channels that are not finite."""
+allowed: boundaries of packed sequences in any order, channels that are not finite,
+states that grow."""
 
 from __future__ import annotations
 
@@ -100,3 +101,60 @@ def test_a_channel_that_is_not_finite_stays_in_its_group(H, G, N, dtype, T, cu, 
             assert torch.equal(got[k][..., 1:], grads[k][..., 1:]), (name, k)
         assert torch.equal(got["A"][1:], grads["A"][1:]) and torch.equal(got["D"][1:], grads["D"][1:])
         assert torch.equal(got["state"][:, 1:], grads["state"][:, 1:])
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_states_that_grow_past_a_chunk(dtype):
+    """Decays above 1 whose product over a chunk is past float32's range: a state of zero
+    stays zero, a small one grows to what it is by definition, and so backward."""
+    dt = R.TYPES[dtype]
+    T, H, N = 200, 3, 4
+    one = torch.ones(1, T, H)
+    t = {"x": torch.zeros(1, T, H), "delta": one.clone(), "A": torch.full((H, N), 2.0),
+         "B": torch.ones(1, T, N), "C": torch.ones(1, T, N)}
+    t["x"][:, -5:] = 0.5
+
+    def dev(kw):
+        return {k: v.to(DEV, v.dtype if k in ("A", "state") else dt).requires_grad_(True) for k, v in kw.items()}
+
+    def run(kw, state=None, go=None, gh=None):
+        kw = dev(kw if state is None else dict(kw, state=state))
+        out, hf = ltc_cuda.ltc_selective_scan(**kw)
+        if go is None and gh is None:
+            return out.detach().cpu().double(), hf.detach().cpu().double()
+        outs, grads = ([out], [go.to(DEV, dt)]) if gh is None else ([hf], [gh.to(DEV)])
+        return dict(zip(kw, torch.autograd.grad(outs, list(kw.values()), grads, allow_unused=True)))
+
+    def definition(kw, state=None):
+        d = {k: v.double() for k, v in kw.items()}
+        return R.scan(d["x"], d["delta"], d["A"], d["B"][:, :, None], d["C"][:, :, None],
+                      state=None if state is None else state.double())
+
+    def close(got, want, steps):
+        # a token's exponent of 3 at most, and its other roundings: 40 a token
+        tol = (40 * steps * 2.0 ** -24 + (R.half_step(dtype) if got.dtype == dt else 0)) * want.abs()
+        return bool(((got.detach().cpu().double() - want).abs() <= tol).all())
+
+    out, hf = run(t)
+    want, whf = definition(t)
+    assert float(out[:, :-5].abs().max()) == 0 and bool(out.isfinite().all())
+    tol = (40 * 5 * 2.0 ** -24 + R.half_step(dtype)) * want.abs()
+    assert bool(((out - want).abs() <= tol).all()) and close(hf, whf, 5)
+    # a state of 1e-30 that grows by e^150 in 100 tokens, the first 64 of which are a chunk
+    small = {k: v[:, :100] if k != "A" else v for k, v in t.items()}
+    small["x"], small["delta"], small["A"] = torch.zeros(1, 100, H), one[:, :100] * 1.5, torch.ones(H, N)
+    state = torch.full((1, H, N), 1e-30)
+    _, hf = run(small, state)
+    assert close(hf, definition(small, state)[1], 100)
+    # backward: a gradient of the first tokens alone, and one of 1e-30 that grows
+    none = dict(t, x=torch.zeros(1, T, H))
+    go = torch.zeros(1, T, H)
+    go[:, :5] = 1.0
+    got = run(none, go=go)
+    gx = torch.zeros(T)
+    for i in range(5):
+        gx[i] = sum(2.718281828459045 ** (2.0 * (j - i)) for j in range(i, 5)) * N
+    assert close(got["x"], gx.double().view(1, T, 1).expand(1, T, H), 5 + 8)
+    assert all(bool(v.isfinite().all()) for v in got.values())
+    got = run(small, torch.zeros(1, H, N), gh=torch.full((1, H, N), 1e-30))
+    assert close(got["state"], torch.full((1, H, N), 2.718281828459045 ** 150 * float(torch.tensor(1e-30))).double(), 100)
