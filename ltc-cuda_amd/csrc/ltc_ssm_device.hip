@@ -539,6 +539,18 @@ __global__ __launch_bounds__(256) void ssm_carry_kernel(SsmArgs p) {
 constexpr int kBE = kSsmBwdStates;  // states of a wave
 constexpr int kBMine = kL / kSsmWavesMax;
 
+// A long sum that carries along what its last addition has lost (Kahan, Further Remarks on
+// Reducing Truncation Errors, 1965): two roundings, however many terms. Of terms that are
+// not finite it is what plain additions give.
+struct Sum {
+  float s = 0.f, over = 0.f;
+  __device__ __forceinline__ void add(float v) {
+    const float y = v - over, t = s + y;
+    over = t - t == 0.f ? (t - s) - y : 0.f;
+    s = t;
+  }
+};
+
 // The sums over the 64 lanes of 64 values a lane, value l's in lane l. Each step halves the
 // values: a lane keeps those whose bit is its own and adds what its partner has of them.
 template <int HALF, int CTRL>
@@ -674,12 +686,13 @@ __global__ __launch_bounds__(64 * kSsmWavesMax) void ssm_bwd_kernel(SsmArgs p) {
   float* s3 = dys + kL * 64 + waves * kL * 64 * 2;           // [waves][kL][64], with z only
   const Work w(p);
   const long long HN = (long long)p.H * p.N;
-  float A2[NG][kBE], g[NG][kBE], dA[NG][kBE];
+  float A2[NG][kBE], g[NG][kBE];
+  Sum dA[NG][kBE];
 #pragma unroll
   for (int r = 0; r < NG; ++r) {
     const int q = r * waves + w.wave;
 #pragma unroll
-    for (int e = 0; e < kBE; ++e) g[r][e] = dA[r][e] = 0.f;
+    for (int e = 0; e < kBE; ++e) g[r][e] = 0.f;
     read_rates<kBE>(p, w, q, A2[r]);
     if (p.chunks > 1)
       states<kBE>(p, w, q, [&](int e, long long at) { g[r][e] = p.ends[w.chunk * HN + at]; });
@@ -690,7 +703,7 @@ __global__ __launch_bounds__(64 * kSsmWavesMax) void ssm_bwd_kernel(SsmArgs p) {
   float skip = p.D != nullptr && w.in ? p.D[w.ch] : 0.f;
   settle(bias);
   settle(skip);
-  float dD = 0.f, dbias = 0.f;
+  Sum dD, dbias;
   const bool gated = p.z != nullptr;
   const int last = w.c0 + (w.c1 - 1 - w.c0) / kL * kL;
   Inputs<T, kBMine> in, next;
@@ -769,7 +782,7 @@ __global__ __launch_bounds__(64 * kSsmWavesMax) void ssm_bwd_kernel(SsmArgs p) {
           advance<i, kBE>(A2[r], bc[r], v[i], h, a[i]);
         });
         if (seg & ed.end) read_states<kBE>(p, w, q, p.gh, t + highest(seg), g[r]);
-        float sums[64];
+        float sums[64], da[kBE] = {};
         back([&](auto i_) {
           constexpr int i = decltype(i_)::value;
           float s1 = 0.f, s2 = 0.f, y = 0.f;
@@ -783,7 +796,7 @@ __global__ __launch_bounds__(64 * kSsmWavesMax) void ssm_bwd_kernel(SsmArgs p) {
             s1 = fmaf(B, d, s1);
             s2 = fmaf(A2[r][e], k, s2);
             y = fmaf(C, ht, y);
-            dA[r][e] = fmaf(v[i].x, k, dA[r][e]);
+            da[e] = fmaf(v[i].x, k, da[e]);
             sums[i * 2 * kBE + e] = d * v[i].y;
             sums[i * 2 * kBE + kBE + e] = dy[i] * ht;
             g[r][e] = ga;
@@ -799,6 +812,8 @@ __global__ __launch_bounds__(64 * kSsmWavesMax) void ssm_bwd_kernel(SsmArgs p) {
             }
           }
         });
+#pragma unroll
+        for (int e = 0; e < kBE; ++e) dA[r][e].add(da[e]);
         if (seg & ed.start) {
           if (p.gs != nullptr)
             at_state(p, t + lowest(seg), [&](long long s) {
@@ -825,6 +840,7 @@ __global__ __launch_bounds__(64 * kSsmWavesMax) void ssm_bwd_kernel(SsmArgs p) {
           p.part_bc[(w.hb * all + (w.g * (long long)pairs + q) * p.ntok + t) * (2 * kBE) + w.lane] = 0.f;
     }
     __syncthreads();
+    float sum_d = 0.f, sum_b = 0.f;
 #pragma unroll
     for (int j = 0; j < kBMine; ++j) {
       const int i = w.wave + j * waves;
@@ -848,8 +864,8 @@ __global__ __launch_bounds__(64 * kSsmWavesMax) void ssm_bwd_kernel(SsmArgs p) {
       if (p.softplus) gd *= sigmoid((float)in.d[j] + bias);
       const float gx = fmaf(dt, s1, skip * dy);
       if (ok) {
-        dD = fmaf(dy, x, dD);
-        dbias += gd;
+        sum_d = fmaf(dy, x, sum_d);
+        sum_b += gd;
       }
       if (p.gx != nullptr) lane_of(static_cast<T*>(p.gx) + at, w.ch) = (T)(ok ? gx : 0.f);
       if (p.gd != nullptr) lane_of(static_cast<T*>(p.gd) + at, w.ch) = (T)(ok ? gd : 0.f);
@@ -859,6 +875,8 @@ __global__ __launch_bounds__(64 * kSsmWavesMax) void ssm_bwd_kernel(SsmArgs p) {
         lane_of(static_cast<T*>(p.gz) + at, w.ch) = (T)(ok ? gz : 0.f);
       }
     }
+    dD.add(sum_d);
+    dbias.add(sum_b);
     in = next;
 #pragma unroll
     for (int r = 0; r < NG; ++r) {
@@ -871,11 +889,11 @@ __global__ __launch_bounds__(64 * kSsmWavesMax) void ssm_bwd_kernel(SsmArgs p) {
   if (p.part_a != nullptr) {
 #pragma unroll
     for (int r = 0; r < NG; ++r)
-      states<kBE>(p, w, r * waves + w.wave, [&](int e, long long at) { p.part_a[w.chunk * HN + at] = dA[r][e]; });
+      states<kBE>(p, w, r * waves + w.wave, [&](int e, long long at) { p.part_a[w.chunk * HN + at] = dA[r][e].s; });
   }
   if (p.part_h != nullptr) {
-    shared[w.wave * 64 + w.lane] = dD;
-    shared[(waves + w.wave) * 64 + w.lane] = dbias;
+    shared[w.wave * 64 + w.lane] = dD.s;
+    shared[(waves + w.wave) * 64 + w.lane] = dbias.s;
     __syncthreads();
     if (w.wave < 2 && w.in) {
       float s = 0.f;
@@ -912,13 +930,13 @@ __global__ __launch_bounds__(256) void ssm_sum_par_kernel(SsmArgs p) {
   const int part = threadIdx.x / kCols;
   const float* from = col < hn ? p.part_a + col : p.part_h + (col - hn);
   const long long stride = col < hn ? hn : 2 * p.H;
-  float s = 0.f;
+  Sum of;
   if (col < cols)
-    for (long long i = part; i < items; i += kParts) s += from[i * stride];
-  sums[part][threadIdx.x % kCols] = s;
+    for (long long i = part; i < items; i += kParts) of.add(from[i * stride]);
+  sums[part][threadIdx.x % kCols] = of.s;
   __syncthreads();
   if (part > 0 || col >= cols) return;
-  s = 0.f;
+  float s = 0.f;
 #pragma unroll
   for (int i = 0; i < kParts; ++i) s += sums[i][threadIdx.x];
   if (col < hn) {

@@ -1,6 +1,6 @@
 """The convolution and the selective scan where their inputs are at an edge of what is
 allowed: boundaries of packed sequences in any order, channels that are not finite,
-states that grow."""
+states that grow, sums over many tokens."""
 
 from __future__ import annotations
 
@@ -158,3 +158,34 @@ def test_states_that_grow_past_a_chunk(dtype):
     assert all(bool(v.isfinite().all()) for v in got.values())
     got = run(small, torch.zeros(1, H, N), gh=torch.full((1, H, N), 1e-30))
     assert close(got["state"], torch.full((1, H, N), 2.718281828459045 ** 150 * float(torch.tensor(1e-30))).double(), 100)
+
+
+@pytest.mark.parametrize("B,T,cu", [(256, 32768, None), (4096, 16, None), (3, 5, None), (1, 70000, None),
+                                    (0, 300000, [0, 100000, 100001, 299999]), (0, 40, [3, 40])])
+def test_sums_over_tokens_do_not_lose_with_their_number(B, T, cu):
+    """The gradients of A, D and the bias add a term a token. Decays of 1 and states of 1
+    make every other operation exact, and every term 1.3: each sum is off by its roundings
+    alone. In units of 2^-24: a batch of 16 tokens 15, the running sum, which carries its
+    error along, 2, eight waves 7 (D and the bias), the blocks 2 and their eight parts 7:
+    33 at most, however many tokens."""
+    n = B * T if cu is None else cu[-1] - cu[0]
+    lead, rows = ((B, T), B) if cu is None else ((T,), len(cu) - 1)
+    c = None if cu is None else torch.tensor(cu, dtype=torch.int32, device=DEV)
+    term = torch.tensor(1.3)
+
+    def full(v, *shape):
+        return torch.full(shape, float(v), device=DEV)
+
+    zero, one = full(0, *lead, 1), full(1, *lead, 1)
+    state, gh = full(1, rows, 1, 1), full(1, rows, 1, 1)
+    want = n * float(term.double())
+
+    def off(x, delta):
+        leaves = {"A": full(0, 1, 1), "D": full(0, 1), "delta_bias": full(0, 1)}
+        leaves = {k: v.requires_grad_(True) for k, v in leaves.items()}
+        out, hf = ltc_cuda.ltc_selective_scan(x, delta, B=one, C=zero, state=state, cu_seqlens=c, **leaves)
+        got = torch.autograd.grad([out, hf], list(leaves.values()), [one, gh])
+        return [abs(float(v.double()) - want) / want / 2.0 ** -24 for v in got]
+
+    errors = [off(zero, one * term.to(DEV))[0], *off(one * term.to(DEV), zero)[1:]]
+    assert max(errors) <= 33, errors
