@@ -155,7 +155,7 @@ struct EmbedArgs {
   // digits; where each id's run begins and ends; sums of pieces
   int* key[2];
   int* pos[2];
-  unsigned* counts;   // [tiles][1 << bits]
+  unsigned* counts;   // [tiles + 1][1 << bits]: of each tile, and of all
   int* begin;         // (V), -1 for an id that does not occur
   int* end;           // (V)
   float* sums;        // [pieces][H]

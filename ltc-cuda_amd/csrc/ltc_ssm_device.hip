@@ -59,11 +59,6 @@ __device__ __forceinline__ float softplus(float v) {
   return fmaxf(v, 0.f) + l;
 }
 
-template <class T>
-__device__ __forceinline__ float value(const T* p) {
-  return (float)*p;
-}
-
 // Element `i` of a row that is the same for the wave: a 32-bit offset of the lane's own
 // leaves the row's address to the scalar unit.
 template <class T>
@@ -265,7 +260,9 @@ __device__ __forceinline__ void advance(const float (&A2)[E], const Coeffs<T, E>
 // sizes of four of a batch's 16 tokens, which the channel's other lanes take from it, and
 // ends with the outputs of these four. So waves neither wait for one another nor share
 // memory, and one wave a SIMD, which is all that many calls have, is kept busy by its own
-// four chains. (64 channels a wave, states over the waves, sums through shared memory with
+// four chains. (In fp32 and for N over 16 the compiler keeps a thread's eight inputs of the
+// first launch in shared memory, 8 KiB a workgroup; no thread reads another's. 64 channels
+// a wave, states over the waves, sums through shared memory with
 // a barrier a batch: B8 T2048 H2048 N16 took 530 us for 1 wave a SIMD.)
 // ---------------------------------------------------------------------------
 constexpr int kFE = 4;                 // states of a lane
@@ -745,7 +742,7 @@ __global__ __launch_bounds__(64 * kSsmWavesMax) void ssm_bwd_kernel(SsmArgs p) {
       dys[i * 64 + w.lane] = ok ? dy : 0.f;
     }
     __syncthreads();
-    // sequence by sequence, from the last, as in the forward
+    // sequence by sequence, from the last
     for (unsigned rest = w.wave < active ? ed.valid : 0u, seg; rest != 0; rest &= ~seg) {
       seg = ed.last(rest);
       float2 v[kL];

@@ -428,6 +428,8 @@ __global__ __launch_bounds__(kThreads) void adjust_kernel(AdjustArgs p) {
   }
   if (p.K == 0) return;
   // The biased logits once more: an id's first entry takes all of its entries, in order.
+  // An entry looks for its id in those before it, load by load: fine for some tens of
+  // biases; for hundreds it outlasts the rest of a small call.
   __syncthreads();
   for (int k = threadIdx.x; k < p.K; k += kThreads) {
     const long long id = id_at(p.bias_ids, p.bias64, row * p.sbi + k);
