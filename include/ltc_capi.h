@@ -498,7 +498,9 @@ int ltc_causal_conv_step(const void* x, long long sxb, const void* weight, const
  *   saved        ltc_selective_scan_saved_floats() floats, written when save is nonzero,
  *                for the backward of the same inputs
  * x, delta, z, B, C, out and their gradients have one type. Tokens outside every sequence
- * give zeros, in out and in the gradients, whatever lies there.
+ * give zeros, in out and in the gradients, whatever lies there. For the backward every
+ * sequence of a batch takes H N floats at least of saved, and as many of workspace, however
+ * short it is; packed sequences do not.
  */
 #define LTC_STATES_MAX 64
 long long ltc_selective_scan_saved_floats(int B, int T, int H, int N, int G, int packed);
